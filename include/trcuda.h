@@ -13,8 +13,8 @@
  *
  * Devices: a function that takes a handle makes the handle's device current on the calling thread
  * (cudaSetDevice) and leaves it current on return; the caller's stream must belong to that device.
- * Functions without a handle (trc_ola, trc_ola_noalloc, trc_remix, trc_resample) run on the calling
- * thread's current device. Restoring a previous device is left to the caller, because doing so from the
+ * Functions without a handle (trc_ola, trc_ola_noalloc, trc_remix, trc_resample, trc_cache_*) run on the
+ * calling thread's current device. Restoring a previous device is left to the caller, because doing so from the
  * library would create a CUDA context on a device the process may never have used.
  *
  * The reference's drop-in surface for this path is the torch op library
@@ -145,6 +145,72 @@ int trc_resample(const float* d_in, int channels, int64_t n_in, int up, int down
 #define TRC_OLA_NOALLOC_MAX_CHUNKS 8192
 int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t* h_starts, int n_chunks,
                     int64_t chunk, int64_t n, float* d_result, void* stream);
+
+/* ------------------------------------------------------------------ frame cache of live input
+ * Keys and values of the frames that live streams have already heard, kept in the pages of a common pool, for a
+ * time attention whose new frames look back over the cache instead of recomputing a whole chunk. The reference
+ * has no counterpart (its attention and rope_pack, kernels.cpp:161-388, take whole chunks); trc_attention and
+ * trc_rope_pack are this library's whole-chunk forms. A push of a few new frames per stream takes three calls:
+ * trc_cache_plan, trc_cache_append, trc_cache_attention, all asynchronous on `stream`, without a handle, without
+ * allocation and without host synchronisation, so they can be captured in a CUDA graph.
+ *
+ * A sequence is one stream; its tokens are frames. A frame's query heads are all bands' heads (heads of band 0,
+ * then of band 1, ...), any number; cache heads divide them evenly (query head i reads cache head
+ * i / (heads / kv_heads)); head dimension 64. Pools: K and V [n_pages][kv_heads][page][64] 16-bit, page 16, 32,
+ * 64 or 128 frames. Block table: int32 [n_seqs][table_stride], entry j the page of frames j * page ...; slot =
+ * page number * page + frame within the page. Rows (new frames) of all sequences are packed: sequence i has rows
+ * cu[i] .. cu[i + 1] - 1, the frames total[i] - (cu[i + 1] - cu[i]) .. total[i] - 1 of its stream. Buffers may be
+ * longer than cu[n_seqs] rows (a captured graph's capacity); the rows behind stay as they were.
+ * Lengths, tables and slots live on the device and are not trusted: bad ones touch no memory outside the
+ * buffers. They set *d_status (int32 on the device, may be NULL) or the plan's flags, and leave the outputs of
+ * the sequences concerned undefined. */
+#define TRC_CACHE_PLAN_MAX_SEQS 8192
+#define TRC_CACHE_MAX_SEQS 2048  /* sequences of one trc_cache_attention */
+#define TRC_CACHE_MAX_GROUP 64   /* query heads per cache head */
+#define TRC_CACHE_NO_PAGES 1     /* plan flags: the free list ran out (missing table entries and slots are -1) */
+#define TRC_CACHE_TABLE_FULL 2   /* a sequence needs more than table_stride pages (its slots there are -1) */
+#define TRC_CACHE_ROWS_FULL 4    /* more new frames than max_rows (rows from max_rows on are not described) */
+#define TRC_CACHE_BAD_LENGTH 8   /* a negative length, or over 2^30 frames in a sequence (taken as 0 and 0) */
+
+/* Block tables, slots and positions of a push. d_cached, d_new [n_seqs]: frames cached and frames to come.
+ * Sequences take the pages they lack, in order, from the front of d_free [n_free] into d_table (in place; other
+ * entries are kept). Writes d_cu [n_seqs + 1], d_total [n_seqs] (cached + new), d_slots and d_positions
+ * [max_rows] (frame number within the stream; rows behind the last get slot -1, position 0) and d_counts [2]:
+ * pages taken from d_free, and the flags above (0 = none). */
+int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, int page, const int32_t* d_free,
+                   int n_free, int32_t* d_table, int table_stride, int max_rows, int32_t* d_cu, int32_t* d_total,
+                   int32_t* d_slots, int32_t* d_positions, int32_t* d_counts, void* stream);
+
+/* trc_rope_pack into the pages. d_qkv: n_rows frames, row_stride elements apart, each of `bands` rows
+ * band_stride elements apart: [heads * 64 q | kv_heads * 64 k | kv_heads * 64 v | heads gate logits (where d_gates
+ * is given)], the output of the unfused qkv+gate GEMM (with bands = 62 and 1544 elements per band row, the
+ * shipped model's). Rotary pairs (2j, 2j + 1) turn by d_positions[row] * d_freqs[j] (fp32 [32], angles in fp64;
+ * NULL: no rotation). d_q [n_rows][bands * heads][64], q_stride elements between frames; k and v go to
+ * d_slots[row] of the pools (bands * kv_heads cache heads); d_gates [n_rows][bands * heads] fp32 = sigmoid
+ * (NULL: none). Rows of slot < 0 are skipped; a slot behind the pool is not written and sets *d_status. Row
+ * starts are multiples of 16 bytes. */
+int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64_t band_stride, int n_rows, int bands,
+                     int heads, int kv_heads, const int32_t* d_positions, const int32_t* d_slots, const float* d_freqs,
+                     int page, int n_pages, void* d_q, int64_t q_stride, void* d_k, void* d_v, float* d_gates,
+                     int* d_status, void* stream);
+
+/* Bytes of d_workspace that trc_cache_attention needs on the current device for these arguments (whatever the
+ * lengths). Negative: an error code. Calls that may overlap on the GPU need workspaces of their own. */
+int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
+
+/* The new frames over their streams' caches: for each row and query head, out = gate * sum_j p_j v_j with
+ * p = softmax(scale q . k_j) over the keys j < total that the masks leave: causal != 0: j <= the row's frame;
+ * window > 0: j > the row's frame - window (0: no limit). A row without keys is zero. d_q and d_out
+ * [n_rows][heads][64] with q_stride / out_stride elements between rows; d_gates [n_rows][heads] fp32 or NULL.
+ * max_new and max_total: the longest new part and the longest total, as far as the host knows them; they choose
+ * between variants and never change which rows and keys are computed. d_workspace is not used where
+ * max_total <= 512. Frames that a row's masks hide do not change it as long as the cached v are finite; what the
+ * pages hold behind `total`, or wholly before every row's window, is not read into any result. */
+int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
+                        const int32_t* d_table, int table_stride, const int32_t* d_cu, const int32_t* d_total,
+                        int n_seqs, int n_rows, int max_new, int max_total, int heads, int kv_heads, int page,
+                        int n_pages, int causal, int window, float scale, const float* d_gates, void* d_out,
+                        int64_t out_stride, void* d_workspace, int64_t workspace_bytes, int* d_status, void* stream);
 
 /* ------------------------------------------------------------------ instrumentation
  * Per-section device timing, the counterpart of the reference's opt-in per-section profile

@@ -2,14 +2,16 @@
 
 Public surface (mirrors the reference package): ``Separator`` (backend="cuda"; ``submit`` for queued
 songs, ``stream`` for live input), ``CudaBSRoformer`` (the FastBSRoformer-compatible forward), the
-chunking helpers, and the device channel fold / resampler (``remix_device``, ``resample_device``).
+chunking helpers, the device channel fold / resampler (``remix_device``, ``resample_device``), and the frame cache
+of live input (``cache_plan``, ``cache_append``, ``cache_attention``).
 """
 
 from .chunking import chunk_starts, hamming, overlap_add, step_for
 from .config import RESURRECTION, TINY, ModelConfig
 
 __all__ = ["Separator", "SeparationJob", "SeparationStream", "CudaBSRoformer", "ModelConfig", "RESURRECTION", "TINY",
-           "chunk_starts", "hamming", "overlap_add", "step_for", "remix_device", "resample_device"]
+           "chunk_starts", "hamming", "overlap_add", "step_for", "remix_device", "resample_device",
+           "CachePlan", "cache_plan", "cache_append", "cache_attention"]
 
 
 def __getattr__(name):
@@ -21,6 +23,10 @@ def __getattr__(name):
         from . import resample
 
         return getattr(resample, name)
+    if name in ("CachePlan", "cache_plan", "cache_append", "cache_attention"):
+        from . import frame_cache
+
+        return getattr(frame_cache, name)
     if name == "CudaBSRoformer":
         from .backend import CudaBSRoformer
 

@@ -73,6 +73,14 @@ SIGNATURES = {
     "trc_remix": (c_int, [c_vp, c_int, c_i64, c_vp, c_vp, c_vp]),
     "trc_resample": (c_int, [c_vp, c_int, c_i64, c_int, c_int, c_i64, c_vp, c_int, c_i64, c_vp, c_vp]),
     "trc_ola_noalloc": (c_int, [c_vp, c_i64, c_vp, c_int, c_i64, c_i64, c_vp, c_vp]),
+    "trc_cache_plan": (c_int, [c_vp, c_vp, c_int, c_int, c_vp, c_int, c_vp, c_int, c_int, c_vp, c_vp, c_vp, c_vp, c_vp,
+                               c_vp]),
+    "trc_cache_append": (c_int, [c_int, c_vp, c_i64, c_i64, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_int, c_int,
+                                 c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "trc_cache_workspace": (c_i64, [c_int, c_int, c_int]),
+    "trc_cache_attention": (c_int, [c_int, c_vp, c_i64, c_vp, c_vp, c_vp, c_int, c_vp, c_vp, c_int, c_int, c_int, c_int,
+                                    c_int, c_int, c_int, c_int, c_int, c_int, c_f, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,
+                                    c_vp]),
     "trc_profile": (c_int, [c_vp, c_int]),
     "trc_profile_read": (c_int, [c_vp, c_char_p, c_int]),
     "trc_launch_count": (ctypes.c_longlong, []),

@@ -101,6 +101,15 @@ int make_map(CUtensorMap* m, int precision, const void* ptr, int rank, const uin
   return TRC_OK;
 }
 
+}  // namespace
+namespace trc {
+int make_tensor_map(CUtensorMap* m, int precision, const void* ptr, int rank, const uint64_t* dims,
+                    const uint64_t* strides_bytes, const uint32_t* box) {
+  return make_map(m, precision, ptr, rank, dims, strides_bytes, box);
+}
+}  // namespace trc
+namespace {
+
 // Cached variant for the forward path (keyed on everything that defines the map).
 int make_map_cached(trc_handle* h, CUtensorMap* m, const void* ptr, int rank, const uint64_t* dims,
                     const uint64_t* strides_bytes, const uint32_t* box, int dtype = -1);

@@ -1,0 +1,197 @@
+// What the attention kernels over the paged frame cache share: the argument block and the division of the
+// work among CTAs.
+//
+// The work is a list of items, one per (sequence, row tile, cache head): a row tile is up to `tpt` new frames
+// with all `group` query heads that share the cache head. An item is a run of 64-key steps that covers the
+// keys some row of it may see. Steps of all items form one line in the order (sequence, row tile, head,
+// step); every CTA takes an equal share of it, whatever the lengths are, so ragged batches, few heads over
+// long caches and many heads over short ones all fill the GPU alike. Where a share ends inside an item the
+// item's parts go to the workspace as (unnormalised sum, maximum, weight) per row and a second kernel joins
+// them in the order of the keys, so results do not depend on timing. A CTA owns two workspace slots: one for
+// a first item begun by another CTA, one for a last item that it begins and does not end.
+// Each CTA derives the line from the device's lengths (a scan over the sequences); the host needs only bounds.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "sm100.cuh"
+
+namespace trc {
+
+constexpr int kCacheMaxSeqs = 2048;
+constexpr int kCacheMaxGroup = 64;
+constexpr int kCacheStep = 64;  // keys per step
+
+struct CacheAttnArgs {
+  const void* q;        // [n_tokens][hq][64] 16-bit, q_stride elements from token to token
+  void* out;            // like q, out_stride
+  int64_t q_stride, out_stride;
+  const float* gates;   // [n_tokens][hq] fp32, or null
+  const int32_t* table; // [n_seqs][table_stride] page numbers
+  const int32_t* cu;    // [n_seqs + 1] first row of each sequence
+  const int32_t* total; // [n_seqs] frames in the cache, the new ones included
+  float* ws;
+  int* status;
+  int n_seqs, n_tokens, hq, hkv, group;
+  int table_stride, page_log2, n_pages;
+  int causal, window;   // window 0: unlimited
+  int split;            // 1: shares may end inside an item
+  int min_share;        // least steps of a share
+  int rows_above, rows_upto;  // this launch's sequences: rows_above < new frames x group <= rows_upto
+  float scale_log2;     // softmax scale x log2(e)
+};
+
+struct CacheSeq {
+  int tok, n, total;  // first row, new frames, frames in the cache
+};
+
+__device__ __forceinline__ CacheSeq cache_seq(const CacheAttnArgs& a, int r) {
+  CacheSeq s;
+  s.tok = min(max(a.cu[r], 0), a.n_tokens);
+  s.n = min(max(a.cu[r + 1], s.tok), a.n_tokens) - s.tok;
+  const int64_t room = min((int64_t)a.table_stride << a.page_log2, (int64_t)1 << 30);
+  s.total = (int)min((int64_t)max(a.total[r], 0), room);
+  const int64_t rows = (int64_t)s.n * a.group;
+  if (rows <= a.rows_above || rows > a.rows_upto) s.n = 0;  // another launch's
+  return s;
+}
+
+// Keys [lo, hi) that new frame i of a sequence sees.
+__device__ __forceinline__ int cache_hi(const CacheAttnArgs& a, const CacheSeq& s, int i) {
+  return a.causal ? min(max(s.total - s.n + i + 1, 0), s.total) : s.total;
+}
+__device__ __forceinline__ int cache_lo(const CacheAttnArgs& a, const CacheSeq& s, int i) {
+  return a.window ? max(s.total - s.n + i + 1 - a.window, 0) : 0;
+}
+
+// One item and its neighbours on the line.
+struct CacheItem {
+  int r, tile, head;  // sequence, row tile, cache head
+  CacheSeq s;
+  int tok0, ntok;     // its new frames (within the sequence)
+  int lo, hi;         // keys that some row sees
+  int t0, t1;         // its steps
+  int64_t start;      // place of its first step on the line
+
+  __device__ __forceinline__ void set_tile(const CacheAttnArgs& a, int tpt) {
+    tok0 = tile * tpt;
+    ntok = min(tpt, s.n - tok0);
+    hi = cache_hi(a, s, tok0 + ntok - 1);
+    lo = min(cache_lo(a, s, tok0), hi);
+    t0 = lo / kCacheStep;
+    t1 = max((hi + kCacheStep - 1) / kCacheStep, t0 + 1);
+  }
+  // the item that holds place `at` (< the line's length); prefix: the line's scan over the sequences
+  __device__ __forceinline__ void seek(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int64_t at) {
+    int x = 0, y = a.n_seqs;  // prefix[x] <= at < prefix[y]
+    while (y - x > 1) {
+      const int m = (x + y) >> 1;
+      if (prefix[m] <= at) x = m; else y = m;
+    }
+    r = x;
+    s = cache_seq(a, r);
+    int64_t left = at - prefix[r];
+    for (tile = 0;; ++tile) {
+      set_tile(a, tpt);
+      const int64_t all = (int64_t)(t1 - t0) * a.hkv;
+      if (left < all) break;
+      left -= all;
+    }
+    head = (int)(left / (t1 - t0));
+    start = at - (left - (int64_t)head * (t1 - t0));
+  }
+  __device__ __forceinline__ void next(const CacheAttnArgs& a, int tpt) {
+    start += t1 - t0;
+    if (++head < a.hkv) return;
+    head = 0;
+    if (tok0 + ntok < s.n) {
+      ++tile;
+    } else {
+      tile = 0;
+      do {
+        if (++r >= a.n_seqs) return;  // the line's end: `start` equals its length
+        s = cache_seq(a, r);
+      } while (s.n == 0);
+    }
+    set_tile(a, tpt);
+  }
+};
+
+// The line's scan, by all `threads` threads of the CTA: prefix[r] = steps before sequence r, prefix[n_seqs] =
+// the line's length. `part` holds 32 int64 of scratch. Ends with a CTA barrier.
+__device__ __forceinline__ void cache_scan(const CacheAttnArgs& a, int tpt, int threads, int64_t* prefix,
+                                           int64_t* part) {
+  const int per = (a.n_seqs + threads - 1) / threads;
+  const int r0 = threadIdx.x * per, r1 = min(r0 + per, a.n_seqs);
+  int64_t sum = 0;
+  for (int r = r0; r < r1; ++r) {
+    CacheItem it;
+    it.s = cache_seq(a, r);
+    int64_t steps = 0;
+    for (it.tile = 0; it.tile * tpt < it.s.n; ++it.tile) {
+      it.set_tile(a, tpt);
+      steps += it.t1 - it.t0;
+    }
+    prefix[r] = sum;
+    sum += steps * a.hkv;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, scan, d);
+    if (lane >= d) scan += o;
+  }
+  if (lane == 31) part[warp] = scan;
+  __syncthreads();
+  int64_t before = scan - sum;
+  for (int w = 0; w < warp; ++w) before += part[w];
+  for (int r = r0; r < r1; ++r) prefix[r] += before;
+  if ((int)threadIdx.x == threads - 1) prefix[a.n_seqs] = before + sum;
+  __syncthreads();
+}
+
+__device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t length, int ctas) {
+  return max((length + ctas - 1) / ctas, (int64_t)a.min_share);
+}
+
+// The runs of steps that one CTA works on, in order.
+struct CacheWalk {
+  CacheItem it;
+  int64_t s0, s1;   // the CTA's share of the line
+  int a0, a1;       // the run's steps [a0, a1) within the item
+  bool valid;
+
+  __device__ __forceinline__ void set_run(const CacheAttnArgs& a) {
+    a0 = it.t0;
+    a1 = it.t1;
+    if (a.split) {
+      if (it.start < s0) a0 += (int)(s0 - it.start);
+      if (it.start + (it.t1 - it.t0) > s1) a1 = it.t0 + (int)(s1 - it.start);
+    }
+  }
+  __device__ __forceinline__ void begin(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int cta, int ctas) {
+    const int64_t length = prefix[a.n_seqs], w = cache_share(a, length, ctas);
+    s0 = min(length, (int64_t)cta * w);
+    s1 = min(length, s0 + w);
+    valid = s0 < s1;
+    if (!valid) return;
+    it.seek(a, tpt, prefix, s0);
+    if (!a.split && it.start < s0) it.next(a, tpt);  // whole items go to the CTA whose share holds their start
+    valid = it.start < s1;
+    if (valid) set_run(a);
+  }
+  __device__ __forceinline__ void advance(const CacheAttnArgs& a, int tpt) {
+    it.next(a, tpt);
+    valid = it.start < s1;
+    if (valid) set_run(a);
+  }
+  __device__ __forceinline__ bool whole() const { return a0 == it.t0 && a1 == it.t1; }
+  __device__ __forceinline__ int slot() const { return a0 == it.t0 ? 1 : 0; }  // of a run that is not whole
+};
+
+// Workspace: slot (2 cta + which) holds [rows][64] sums, then [rows][2] (maximum in log2 units, weight).
+__host__ __device__ __forceinline__ int64_t cache_slot_floats(int rows) { return (int64_t)rows * 66; }
+
+}  // namespace trc

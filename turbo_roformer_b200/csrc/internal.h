@@ -13,6 +13,12 @@ struct MlpArgs;
 
 // api.cu: adds kernels launched outside api.cu to the count trc_launch_count reports
 void count_launches(int n);
+// api.cu: records the calling thread's error message and returns `code`
+int set_last_error(int code, const char* msg);
+// api.cu: tensor map of a row-major tensor (dims[0] innermost, strides in bytes for the others) with the 128-byte
+// swizzle; precision 0 fp16, 1 bf16. TRC_OK or an error code.
+int make_tensor_map(CUtensorMap* m, int precision, const void* ptr, int rank, const uint64_t* dims,
+                    const uint64_t* strides_bytes, const uint32_t* box);
 
 // dsp.cu
 void launch_stft(const float* audio, int B, int64_t L, int T, int n, int hop, const float* window, const float2* tw,
