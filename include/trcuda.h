@@ -167,6 +167,7 @@ int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t*
 #define TRC_CACHE_PLAN_MAX_SEQS 8192
 #define TRC_CACHE_MAX_SEQS 2048  /* sequences of one trc_cache_attention */
 #define TRC_CACHE_MAX_GROUP 64   /* query heads per cache head */
+#define TRC_CACHE_MAX_WHOLE 512  /* up to this max_total, trc_cache_attention uses no workspace */
 #define TRC_CACHE_NO_PAGES 1     /* plan flags: the free list ran out (missing table entries and slots are -1) */
 #define TRC_CACHE_TABLE_FULL 2   /* a sequence needs more than table_stride pages (its slots there are -1) */
 #define TRC_CACHE_ROWS_FULL 4    /* more new frames than max_rows (rows from max_rows on are not described) */
@@ -204,7 +205,7 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
  * [n_rows][heads][64] with q_stride / out_stride elements between rows; d_gates [n_rows][heads] fp32 or NULL.
  * max_new and max_total: the longest new part and the longest total, as far as the host knows them; they choose
  * between variants and never change which rows and keys are computed. d_workspace is not used where
- * max_total <= 512. Frames that a row's masks hide do not change it as long as the cached v are finite; what the
+ * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are finite; what the
  * pages hold behind `total`, or wholly before every row's window, is not read into any result. */
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
                         const int32_t* d_table, int table_stride, const int32_t* d_cu, const int32_t* d_total,

@@ -14,6 +14,7 @@
 
 #include "../../include/trcuda.h"
 #include "cache_attention.cuh"
+#include "cache_attention_long.cuh"
 #include "cache_sched.cuh"
 #include "internal.h"
 
@@ -340,40 +341,91 @@ int sm_count() {
 int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 constexpr int kCtasPerSm = 2;
+constexpr int kLongRows = 128;  // rows per (sequence, cache head) above which the tcgen05 kernel takes a sequence
+
+// Dynamic shared-memory opt-in, once per kernel and device (`done`: one object per kernel).
+template <typename Kern>
+int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit);
+  }
+  return e == cudaSuccess ? TRC_OK : set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
+}
+
+template <typename T>
+int launch_join(const CacheAttnArgs& a, int rows, int ctas, cudaStream_t st) {
+  if (!a.split) return TRC_OK;
+  cache_join_kernel<T><<<dim3(ctas, rows > 32 ? 4 : 1), 256, 0, st>>>(a, rows);
+  return launched("cache attention join", 1);
+}
 
 template <typename T, int MT, int WM, int WK, int KT, int ST>
 int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int ctas, cudaStream_t st) {
   using S = CacheRowsSmem<MT, WM, WK, KT, ST>;
   auto kern = cache_rows_kernel<T, MT, WM, WK, KT, ST>;
   static std::atomic<unsigned long long> done{0};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const unsigned long long bit = 1ull << (dev & 63);
-  if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(kCacheMaxSeqs));
-    if (e == cudaSuccess) done.fetch_or(bit);
-  }
-  if (e != cudaSuccess) return set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
+  int rc = allow_smem(kern, S::bytes(kCacheMaxSeqs), done);
+  if (rc) return rc;
   kern<<<ctas, 32 * WM * WK, S::bytes(a.n_seqs), st>>>(mk, mv, a);
-  int rc = launched("cache attention", 1);
-  if (rc || !a.split) return rc;
-  constexpr int rows = 16 * MT * WM;
-  cache_join_kernel<T><<<dim3(ctas, (rows + 7) / 8), 256, (32 + a.n_seqs + 1) * 8, st>>>(a, rows, ctas);
-  return launched("cache attention join", 1);
+  rc = launched("cache attention", 1);
+  return rc ? rc : launch_join<T>(a, 16 * MT * WM, ctas, st);
+}
+
+// The tcgen05 kernel moves registers between its warpgroups (setmaxnreg): the split must fit in what the launch gives
+// the block, or the softmax warps' increase would never be granted.
+template <typename T>
+int launch_long(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int ctas, cudaStream_t st) {
+  auto kern = cache_long_kernel<T>;
+  static std::atomic<unsigned long long> done{0};
+  int rc = allow_smem(kern, ClSmem::bytes(kCacheMaxSeqs), done);
+  if (rc) return rc;
+  static std::atomic<int> regs{0};
+  if (regs.load() == 0) {
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
+    regs.store(fa.numRegs);
+  }
+  if (4 * 32 * kTaRegsLow + 12 * 32 * kTaRegsHigh > kTaThreads * regs.load())
+    return set_last_error(TRC_E_CUDA, "cache attention: register split larger than the launch's registers");
+  CUtensorMap mq;
+  const uint64_t dims[3] = {64, (uint64_t)a.hq, (uint64_t)a.n_tokens};
+  const uint64_t strides[2] = {128, 2 * (uint64_t)(a.n_tokens > 1 ? a.q_stride : (int64_t)a.hq * 64)};
+  const uint32_t box[3] = {64, (uint32_t)a.group, (uint32_t)(128 / a.group)};
+  if ((rc = make_tensor_map(&mq, OperandType<T>::kFormat, a.q, 3, dims, strides, box))) return rc;
+  kern<<<ctas, kTaThreads, ClSmem::bytes(a.n_seqs), st>>>(mq, mk, mv, a);
+  rc = launched("cache attention", 1);
+  return rc ? rc : launch_join<T>(a, kClRows, ctas, st);
 }
 
 template <typename T>
-int launch_cache_attention(int rows, int page, const void* k, const void* v, CacheAttnArgs a, int ctas,
+int launch_cache_attention(int64_t most_rows, int page, const void* k, const void* v, CacheAttnArgs a, int sms,
                            cudaStream_t st) {
   const int prec = OperandType<T>::kFormat;
-  const int keys = rows <= 16 ? 32 : 64;
   const uint64_t dims[2] = {64, (uint64_t)a.n_pages * a.hkv * page};
   const uint64_t strides[1] = {128};
-  const uint32_t box[2] = {64, (uint32_t)(page < keys ? page : keys)};
+  auto maps = [&](uint32_t keys, CUtensorMap& mk, CUtensorMap& mv) {
+    const uint32_t box[2] = {64, (uint32_t)page < keys ? (uint32_t)page : keys};
+    const int rc = make_tensor_map(&mk, prec, k, 2, dims, strides, box);
+    return rc ? rc : make_tensor_map(&mv, prec, v, 2, dims, strides, box);
+  };
   CUtensorMap mk, mv;
-  int rc = make_tensor_map(&mk, prec, k, 2, dims, strides, box);
-  if (!rc) rc = make_tensor_map(&mv, prec, v, 2, dims, strides, box);
-  if (rc) return rc;
+  int rc;
+  const int ctas = kCtasPerSm * sms;
+  if (most_rows > kLongRows) {
+    if ((rc = maps(64, mk, mv))) return rc;
+    a.rows_above = kLongRows;
+    if ((rc = launch_long<T>(mk, mv, a, sms, st))) return rc;
+    a.rows_above = 0;
+    a.rows_upto = kLongRows;
+    return launch_rows<T, 2, 4, 1, 64, 6>(mk, mv, a, ctas, st);
+  }
+  const int rows = tile_rows(most_rows);
+  if ((rc = maps(rows <= 16 ? 32 : 64, mk, mv))) return rc;
   // stages: 96 KB per CTA, two CTAs per SM
   switch (rows) {
     case 16: return launch_rows<T, 1, 1, 4, 32, 3>(mk, mv, a, ctas, st);
@@ -500,8 +552,12 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads) {
     return set_last_error(TRC_E_INVALID, "cache workspace: bad sizes");
   const int sms = trc::sm_count();
   if (!sms) return set_last_error(TRC_E_CUDA, "cache workspace: no current CUDA device");
-  const int rows = trc::tile_rows((int64_t)(max_new > 0 ? max_new : 1) * (heads / kv_heads));
-  return 2ll * trc::kCtasPerSm * sms * trc::cache_slot_floats(rows) * 4;
+  const int64_t most = (int64_t)(max_new > 0 ? max_new : 1) * (heads / kv_heads);
+  // launches of one call follow one another on its stream and share the workspace
+  int64_t floats = trc::cache_workspace_floats(trc::tile_rows(most), trc::kCtasPerSm * sms);
+  if (most > trc::kLongRows && trc::cache_workspace_floats(trc::kClRows, sms) > floats)
+    floats = trc::cache_workspace_floats(trc::kClRows, sms);
+  return 4 * floats;
 }
 
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
@@ -561,18 +617,17 @@ int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const 
   a.rows_above = 0;
   a.rows_upto = INT_MAX;
   a.min_share = 4;
-  a.split = max_total > 512;
-  const int rows = trc::tile_rows((int64_t)(max_new > 0 ? max_new : 1) * a.group);
+  a.split = max_total > TRC_CACHE_MAX_WHOLE;
+  const int64_t most = (int64_t)(max_new > 0 ? max_new : 1) * a.group;
   if (a.split) {
     if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 16 ||
         workspace_bytes < trc_cache_workspace(max_new, heads, kv_heads))
       return set_last_error(TRC_E_INVALID, "cache attention: workspace missing or smaller than trc_cache_workspace");
   }
   cudaStream_t st = (cudaStream_t)stream;
-  const int ctas = trc::kCtasPerSm * sms;
   return precision == TRC_PREC_FP16
-             ? trc::launch_cache_attention<__half>(rows, page, d_k, d_v, a, ctas, st)
-             : trc::launch_cache_attention<__nv_bfloat16>(rows, page, d_k, d_v, a, ctas, st);
+             ? trc::launch_cache_attention<__half>(most, page, d_k, d_v, a, sms, st)
+             : trc::launch_cache_attention<__nv_bfloat16>(most, page, d_k, d_v, a, sms, st);
 }
 
 }  // extern "C"

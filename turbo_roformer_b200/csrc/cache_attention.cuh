@@ -101,10 +101,11 @@ __global__ void __launch_bounds__(32 * WM * WK, 2)
     tma_prefetch_desc(&map_v);
   }
   const int tpt = kRows / args.group;
-  cache_scan(args, tpt, kThreads, prefix, part);  // its barriers cover the initialisation above
+  const bool split = cache_scan(args, tpt, kThreads, gridDim.x, prefix, part);  // its barriers cover the above
 
   CacheWalk cons;
-  cons.begin(args, tpt, prefix, blockIdx.x, gridDim.x);
+  cons.begin(args, tpt, prefix, blockIdx.x, gridDim.x, split);
+  if (args.split && threadIdx.x == 0) cache_record(args, blockIdx.x)->parts = 0;
   if (!cons.valid) return;
   bool ok = true;
 
@@ -377,7 +378,9 @@ __global__ void __launch_bounds__(32 * WM * WK, 2)
     // ---- results, or this run's part of them
     if (wk == 0) {
       const bool whole = cons.whole();
-      float* slot = whole ? nullptr : args.ws + cache_slot_floats(kRows) * (2 * (int64_t)blockIdx.x + cons.slot());
+      float* slot = whole ? nullptr : cache_slot(args, kRows, gridDim.x, 2 * blockIdx.x + cons.slot());
+      if (!whole && cons.slot() == 1 && threadIdx.x == 0)
+        *cache_record(args, blockIdx.x) = {cons.parts(), it.s.tok + it.tok0, it.ntok, it.head};
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -411,41 +414,28 @@ __global__ void __launch_bounds__(32 * WM * WK, 2)
   }
 }
 
-// Joins the parts of items that were divided among CTAs. Block (c, y) takes the item that CTA c began and did
-// not end; its warps take rows y * 8 .. y * 8 + 7. A warp reads two parts at a time (16 lanes x 4 dims each).
+// Joins the parts of items that were divided among CTAs. Blocks (c, y) take the item that CTA c began and did not
+// end, if there is one; their warps take its rows in turn. A warp reads two parts at a time (16 lanes x 4 dims).
 template <typename T>
-__global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__ CacheAttnArgs args, int tile_rows,
-                                                         int ctas) {
-  extern __shared__ int64_t join_smem[];
-  int64_t* part = join_smem;
-  int64_t* prefix = join_smem + 32;
-  const int tpt = tile_rows / args.group;
-  cache_scan(args, tpt, 256, prefix, part);
-  const int64_t length = prefix[args.n_seqs], share = cache_share(args, length, ctas);
-  const int64_t s0 = share * blockIdx.x, s1 = s0 + share;
-  if (s1 >= length) return;
-  CacheItem it;
-  it.seek(args, tpt, prefix, s1);
-  if (it.start >= s1 || it.start < s0) return;  // none, or begun by an earlier CTA
-  const int parts = 1 + (int)((it.start + (it.t1 - it.t0) - 1) / share) - (int)blockIdx.x;
-  const int row = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= it.ntok * args.group) return;
-  const int sub = lane >> 4, d = (lane & 15) * 4;
-  const int64_t slot = cache_slot_floats(tile_rows);
-  float m = -INFINITY, l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+__global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__ CacheAttnArgs args, int tile_rows) {
+  const int ctas = gridDim.x;
+  const CacheRecord rec = *cache_record(args, blockIdx.x);
+  if (rec.parts == 0) return;
+  const int lane = threadIdx.x & 31, sub = lane >> 4, d = (lane & 15) * 4;
+  for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < rec.ntok * args.group; row += gridDim.y * 8) {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int p = sub; p < parts; p += 2) {
-    const float* src = args.ws + slot * (2 * ((int64_t)blockIdx.x + p) + (p == 0 ? 1 : 0));
-    const float2 ml = *reinterpret_cast<const float2*>(src + tile_rows * 64 + row * 2);
-    const float4 x = *reinterpret_cast<const float4*>(src + row * 64 + d);
-    const float mn = fmaxf(m, ml.x);
-    const float f1 = mn == -INFINITY ? 1.f : ex2_approx(m - mn), f2 = mn == -INFINITY ? 1.f : ex2_approx(ml.x - mn);
-    m = mn;
-    l = l * f1 + ml.y * f2;
-    o = make_float4(o.x * f1 + x.x * f2, o.y * f1 + x.y * f2, o.z * f1 + x.z * f2, o.w * f1 + x.w * f2);
-  }
-  {
+    for (int p = sub; p < rec.parts; p += 2) {
+      const float* src = cache_slot(args, tile_rows, ctas, 2 * (blockIdx.x + p) + (p == 0 ? 1 : 0));
+      const float2 ml = *reinterpret_cast<const float2*>(src + tile_rows * 64 + row * 2);
+      const float4 x = *reinterpret_cast<const float4*>(src + row * 64 + d);
+      const float mn = fmaxf(m, ml.x);
+      const float f1 = mn == -INFINITY ? 1.f : ex2_approx(m - mn), f2 = mn == -INFINITY ? 1.f : ex2_approx(ml.x - mn);
+      m = mn;
+      l = l * f1 + ml.y * f2;
+      o = make_float4(o.x * f1 + x.x * f2, o.y * f1 + x.y * f2, o.z * f1 + x.z * f2, o.w * f1 + x.w * f2);
+    }
     const float m2 = __shfl_xor_sync(0xffffffffu, m, 16), l2 = __shfl_xor_sync(0xffffffffu, l, 16);
     const float mn = fmaxf(m, m2);
     const float f1 = mn == -INFINITY ? 1.f : ex2_approx(m - mn), f2 = mn == -INFINITY ? 1.f : ex2_approx(m2 - mn);
@@ -454,16 +444,17 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
     o.y = o.y * f1 + __shfl_xor_sync(0xffffffffu, o.y, 16) * f2;
     o.z = o.z * f1 + __shfl_xor_sync(0xffffffffu, o.z, 16) * f2;
     o.w = o.w * f1 + __shfl_xor_sync(0xffffffffu, o.w, 16) * f2;
+    if (sub == 0) {
+      const int i = row / args.group, head = rec.head * args.group + (row - i * args.group);
+      const int64_t tok = rec.tok + i;
+      const float gate = args.gates ? args.gates[tok * args.hq + head] : 1.f;
+      const float f = l == 0.f ? 0.f : gate / l;
+      uint2 u;
+      u.x = OperandType<T>::pack2(o.x * f, o.y * f);
+      u.y = OperandType<T>::pack2(o.z * f, o.w * f);
+      *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + tok * args.out_stride + head * 64 + d) = u;
+    }
   }
-  if (sub) return;
-  const int i = row / args.group, head = it.head * args.group + (row - i * args.group);
-  const int64_t tok = it.s.tok + it.tok0 + i;
-  const float gate = args.gates ? args.gates[tok * args.hq + head] : 1.f;
-  const float f = l == 0.f ? 0.f : gate / l;
-  uint2 u;
-  u.x = OperandType<T>::pack2(o.x * f, o.y * f);
-  u.y = OperandType<T>::pack2(o.z * f, o.w * f);
-  *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + tok * args.out_stride + head * 64 + d) = u;
 }
 
 }  // namespace trc

@@ -118,13 +118,21 @@ struct CacheItem {
   }
 };
 
+// A CTA's share of a line of `length` steps.
+__device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t length, int ctas) {
+  return max((length + ctas - 1) / ctas, (int64_t)a.min_share);
+}
+
 // The line's scan, by all `threads` threads of the CTA: prefix[r] = steps before sequence r, prefix[n_seqs] =
-// the line's length. `part` holds 32 int64 of scratch. Ends with a CTA barrier.
-__device__ __forceinline__ void cache_scan(const CacheAttnArgs& a, int tpt, int threads, int64_t* prefix,
+// the line's length. Returns whether shares end inside items: not where the host rules it out, nor where a share
+// holds at least 16 of the longest items (whole items are then at most 1/16 uneven, and there is nothing to join).
+// `part` holds 32 int64 of scratch. Ends with a CTA barrier.
+__device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int threads, int ctas, int64_t* prefix,
                                            int64_t* part) {
   const int per = (a.n_seqs + threads - 1) / threads;
-  const int r0 = threadIdx.x * per, r1 = min(r0 + per, a.n_seqs);
+  const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
   int64_t sum = 0;
+  int longest = 0;
   for (int r = r0; r < r1; ++r) {
     CacheItem it;
     it.s = cache_seq(a, r);
@@ -132,6 +140,7 @@ __device__ __forceinline__ void cache_scan(const CacheAttnArgs& a, int tpt, int 
     for (it.tile = 0; it.tile * tpt < it.s.n; ++it.tile) {
       it.set_tile(a, tpt);
       steps += it.t1 - it.t0;
+      longest = max(longest, it.t1 - it.t0);
     }
     prefix[r] = sum;
     sum += steps * a.hkv;
@@ -145,53 +154,73 @@ __device__ __forceinline__ void cache_scan(const CacheAttnArgs& a, int tpt, int 
   }
   if (lane == 31) part[warp] = scan;
   __syncthreads();
-  int64_t before = scan - sum;
-  for (int w = 0; w < warp; ++w) before += part[w];
+  int64_t before = scan - sum, length = 0;
+  for (int w = 0; w < threads / 32; ++w) {
+    if (w < warp) before += part[w];
+    length += part[w];
+  }
   for (int r = r0; r < r1; ++r) prefix[r] += before;
-  if ((int)threadIdx.x == threads - 1) prefix[a.n_seqs] = before + sum;
-  __syncthreads();
-}
-
-__device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t length, int ctas) {
-  return max((length + ctas - 1) / ctas, (int64_t)a.min_share);
+  if (threadIdx.x == 0) prefix[a.n_seqs] = length;
+  return __syncthreads_or(a.split && longest * (int64_t)16 > cache_share(a, length, ctas));
 }
 
 // The runs of steps that one CTA works on, in order.
 struct CacheWalk {
   CacheItem it;
-  int64_t s0, s1;   // the CTA's share of the line
-  int a0, a1;       // the run's steps [a0, a1) within the item
-  bool valid;
+  int64_t s0, s1;  // the CTA's share of the line
+  int a0, a1;      // the run's steps [a0, a1) within the item
+  bool split, valid;
 
-  __device__ __forceinline__ void set_run(const CacheAttnArgs& a) {
+  __device__ __forceinline__ void set_run() {
     a0 = it.t0;
     a1 = it.t1;
-    if (a.split) {
+    if (split) {
       if (it.start < s0) a0 += (int)(s0 - it.start);
       if (it.start + (it.t1 - it.t0) > s1) a1 = it.t0 + (int)(s1 - it.start);
     }
   }
-  __device__ __forceinline__ void begin(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int cta, int ctas) {
+  __device__ __forceinline__ void begin(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int cta, int ctas,
+                                        bool divided) {
     const int64_t length = prefix[a.n_seqs], w = cache_share(a, length, ctas);
+    split = divided;
     s0 = min(length, (int64_t)cta * w);
     s1 = min(length, s0 + w);
     valid = s0 < s1;
     if (!valid) return;
     it.seek(a, tpt, prefix, s0);
-    if (!a.split && it.start < s0) it.next(a, tpt);  // whole items go to the CTA whose share holds their start
+    if (!split && it.start < s0) it.next(a, tpt);  // whole items go to the CTA whose share holds their start
     valid = it.start < s1;
-    if (valid) set_run(a);
+    if (valid) set_run();
   }
   __device__ __forceinline__ void advance(const CacheAttnArgs& a, int tpt) {
     it.next(a, tpt);
     valid = it.start < s1;
-    if (valid) set_run(a);
+    if (valid) set_run();
   }
   __device__ __forceinline__ bool whole() const { return a0 == it.t0 && a1 == it.t1; }
   __device__ __forceinline__ int slot() const { return a0 == it.t0 ? 1 : 0; }  // of a run that is not whole
+  // CTAs that work on this item, when it is begun here and not ended
+  __device__ __forceinline__ int parts() const {
+    const int64_t w = s1 - s0;  // a share that an item outlasts is not the line's last, so it is a full one
+    return 1 + (int)((it.start + (it.t1 - it.t0) - 1 - s0) / w);
+  }
 };
 
-// Workspace: slot (2 cta + which) holds [rows][64] sums, then [rows][2] (maximum in log2 units, weight).
+// Workspace: for each CTA a record of the item that it begins and does not end, then the slots. Slot
+// (2 cta + which) holds [rows][64] sums, then [rows][2] (maximum in log2 units, weight).
+struct CacheRecord {
+  int parts;  // CTAs that work on the item; 0: there is none
+  int tok, ntok, head;
+};
 __host__ __device__ __forceinline__ int64_t cache_slot_floats(int rows) { return (int64_t)rows * 66; }
+__host__ __device__ __forceinline__ int64_t cache_workspace_floats(int rows, int ctas) {
+  return 4ll * ctas + 2ll * ctas * cache_slot_floats(rows);
+}
+__device__ __forceinline__ CacheRecord* cache_record(const CacheAttnArgs& a, int cta) {
+  return reinterpret_cast<CacheRecord*>(a.ws) + cta;
+}
+__device__ __forceinline__ float* cache_slot(const CacheAttnArgs& a, int rows, int ctas, int slot) {
+  return a.ws + 4ll * ctas + cache_slot_floats(rows) * slot;
+}
 
 }  // namespace trc

@@ -25,6 +25,7 @@ from . import _lib
 HEAD_DIM = 64
 PAGES = (16, 32, 64, 128)
 _PRECISION = {torch.float16: _lib.TRC_PREC_FP16, torch.bfloat16: _lib.TRC_PREC_BF16}
+MAX_WHOLE = 512  # TRC_CACHE_MAX_WHOLE: up to this max_total trc_cache_attention takes no workspace
 _INT32_MAX = 2**31 - 1
 
 
@@ -38,57 +39,60 @@ class CachePlan(NamedTuple):
     counts: torch.Tensor     # (2,) pages taken from the free list; TRC_CACHE_* flags, 0 for none
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
+def _ints(t: torch.Tensor, index: int, ndim: int, name: str) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != index or t.ndim != ndim or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {ndim}-d int32 tensor on cuda:{index}")
 
 
-def _ints(t: torch.Tensor, device: torch.device, ndim: int, name: str) -> None:
-    if t.dtype != torch.int32 or t.device != device or t.ndim != ndim or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {ndim}-d int32 tensor on {device}")
-
-
-def _status_ptr(status: torch.Tensor | None, device: torch.device) -> int:
+def _status_ptr(status: torch.Tensor | None, index: int) -> int:
     if status is None:
         return 0
-    if status.dtype != torch.int32 or status.device != device or status.numel() != 1:
-        raise ValueError(f"status must be an int32 tensor of one element on {device}")
+    if status.dtype is not torch.int32 or status.get_device() != index or status.numel() != 1:
+        raise ValueError(f"status must be an int32 tensor of one element on cuda:{index}")
     return status.data_ptr()
 
 
-def _call(device: torch.device, fn: str, *args) -> None:
-    """fn(*args, stream) with `device` current (it is set and put back only where another one is)."""
+def _call(index: int, fn: str, *args) -> None:
+    """fn(*args, stream) on device `index` and its current stream (made current only where another device is)."""
     lib = _lib.load()
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+    # the raw handle of torch.cuda.current_stream(index), without the Stream object around it (a pass's latency)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
         rc = getattr(lib, fn)(*args, stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             rc = getattr(lib, fn)(*args, stream)
     if rc:
         _lib.check(rc)
 
 
-def _pools(k: torch.Tensor, v: torch.Tensor, device: torch.device, dtype: torch.dtype) -> tuple[int, int, int]:
+def _pools(k: torch.Tensor, v: torch.Tensor, index: int, dtype: torch.dtype) -> tuple[int, int, int]:
     """(pages, cache heads, frames per page) of a pool pair."""
-    if k.ndim != 4 or k.shape != v.shape or k.shape[3] != HEAD_DIM or k.shape[2] not in PAGES:
+    shape = k.shape
+    if len(shape) != 4 or shape != v.shape or shape[3] != HEAD_DIM or shape[2] not in PAGES:
         raise ValueError("pools must be (pages, cache heads, 16 | 32 | 64 | 128, 64), k and v alike")
-    if k.dtype != dtype or v.dtype != dtype or k.device != device or v.device != device:
-        raise ValueError(f"pools must be {dtype} on {device}")
+    if k.dtype is not dtype or v.dtype is not dtype or k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"pools must be {dtype} on cuda:{index}")
     if not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("pools must be contiguous")
-    return k.shape[0], k.shape[1], k.shape[2]
+    return shape[0], shape[1], shape[2]
 
 
-def _row_stride(t: torch.Tensor, shape: tuple[int, int, int], device: torch.device, dtype: torch.dtype,
-                name: str) -> int:
+def _row_stride(t: torch.Tensor, rows: int, heads: int, index: int, dtype: torch.dtype, name: str) -> int:
     """Elements between rows of a (rows, heads, 64) tensor whose rows are contiguous."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name} must be {shape} {dtype} on {device}")
+    if t.shape != (rows, heads, HEAD_DIM) or t.dtype is not dtype or t.get_device() != index:
+        raise ValueError(f"{name} must be ({rows}, {heads}, {HEAD_DIM}) {dtype} on cuda:{index}")
     st = t.stride()
-    if st[2] != 1 or (shape[1] > 1 and st[1] != HEAD_DIM):
+    if st[2] != 1 or (heads > 1 and st[1] != HEAD_DIM):
         raise ValueError(f"{name}: a row's heads must be contiguous")
-    return st[0] if shape[0] > 1 else shape[1] * HEAD_DIM
+    return st[0] if rows > 1 else heads * HEAD_DIM
+
+
+def _gates_ptr(gates: torch.Tensor, rows: int, heads: int, index: int) -> int:
+    if (gates.shape != (rows, heads) or gates.dtype is not torch.float32 or gates.get_device() != index
+            or not gates.is_contiguous()):
+        raise ValueError(f"gates must be a contiguous ({rows}, {heads}) float32 tensor on cuda:{index}")
+    return gates.data_ptr()
 
 
 def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, page: int,
@@ -96,29 +100,33 @@ def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, fre
     """Pages, slots and positions of a push: ``cached`` and ``new`` (sequences,) int32 frames each sequence has and
     gets. Sequences take the pages they lack from the front of ``free_pages`` into ``table`` (sequences, columns),
     in place; ``max_rows`` is the capacity of the per-row outputs. ``out``: a plan to write into."""
-    device = cached.device
-    _need(cached.is_cuda, "cached must be a CUDA tensor")
-    _ints(cached, device, 1, "cached")
-    _ints(new, device, 1, "new")
-    _ints(table, device, 2, "table")
-    _ints(free_pages, device, 1, "free_pages")
+    if not cached.is_cuda:
+        raise ValueError("cached must be a CUDA tensor")
+    index = cached.get_device()
+    _ints(cached, index, 1, "cached")
+    _ints(new, index, 1, "new")
+    _ints(table, index, 2, "table")
+    _ints(free_pages, index, 1, "free_pages")
     n = cached.shape[0]
-    _need(new.shape[0] == n and table.shape[0] == n, "cached, new and table must agree in the number of sequences")
-    _need(page in PAGES, f"page must be one of {PAGES}")
-    _need(0 <= max_rows <= _INT32_MAX, "max_rows out of range")
+    rows, columns = table.shape
+    if new.shape[0] != n or rows != n:
+        raise ValueError("cached, new and table must agree in the number of sequences")
+    if page not in PAGES:
+        raise ValueError(f"page must be one of {PAGES}")
+    if not 0 <= max_rows <= _INT32_MAX:
+        raise ValueError("max_rows out of range")
+    sizes = (n + 1, n, max_rows, max_rows, 2)
     if out is None:
-        # one allocation, the arrays on 16-byte boundaries
-        sizes = (n + 1, n, max_rows, max_rows, 2)
-        up = [(x + 3) & ~3 for x in sizes]
-        out = CachePlan(*(p[:x] for p, x in zip(torch.empty(sum(up), dtype=torch.int32, device=device).split(up),
-                                                sizes)))
+        out = CachePlan(*cached.new_empty(sum(sizes)).split_with_sizes(sizes))  # one allocation
     else:
-        for t, size, name in zip(out, (n + 1, n, max_rows, max_rows, 2), CachePlan._fields):
-            _ints(t, device, 1, name)
-            _need(t.shape[0] == size, f"{name} must have {size} elements")
-    _call(device, "trc_cache_plan", cached.data_ptr(), new.data_ptr(), n, page, free_pages.data_ptr(),
-          free_pages.shape[0], table.data_ptr(), table.shape[1], max_rows, out.cu.data_ptr(), out.total.data_ptr(),
-          out.slots.data_ptr(), out.positions.data_ptr(), out.counts.data_ptr())
+        for t, size, name in zip(out, sizes, CachePlan._fields):
+            _ints(t, index, 1, name)
+            if t.shape[0] != size:
+                raise ValueError(f"{name} must have {size} elements")
+    cu, total, slots, positions, counts = out
+    _call(index, "trc_cache_plan", cached.data_ptr(), new.data_ptr(), n, page, free_pages.data_ptr(),
+          free_pages.shape[0], table.data_ptr(), columns, max_rows, cu.data_ptr(), total.data_ptr(), slots.data_ptr(),
+          positions.data_ptr(), counts.data_ptr())
     return out
 
 
@@ -134,44 +142,52 @@ def cache_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     64) and the sigmoid gates (rows, bands * heads) fp32, or None; ``q`` and ``gates`` may be tensors to write into
     (``gates=True``: a new one). Rows whose slot is -1 are skipped: where q and gates are new, their values there
     are undefined."""
-    device, dtype = qkv.device, qkv.dtype
-    _need(qkv.is_cuda and qkv.ndim == 3 and dtype in _PRECISION, "qkv must be a (rows, bands, width) fp16 or bf16 CUDA tensor")
+    dtype = qkv.dtype
+    if not qkv.is_cuda or qkv.ndim != 3 or dtype not in _PRECISION:
+        raise ValueError("qkv must be a (rows, bands, width) fp16 or bf16 CUDA tensor")
+    index = qkv.get_device()
     rows, bands, width = qkv.shape
-    _need(heads >= 1 and kv_heads >= 1 and heads % kv_heads == 0, "kv_heads must divide heads")
-    n_pages, cache_heads, page = _pools(k_pages, v_pages, device, dtype)
-    _need(bands >= 1 and cache_heads == bands * kv_heads, "the pools must have bands * kv_heads cache heads")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("kv_heads must divide heads")
+    n_pages, cache_heads, page = _pools(k_pages, v_pages, index, dtype)
+    if bands < 1 or cache_heads != bands * kv_heads:
+        raise ValueError("the pools must have bands * kv_heads cache heads")
     wanted = gates is not None and gates is not False
-    _need(width >= (heads + 2 * kv_heads) * HEAD_DIM + (heads if wanted else 0), "qkv rows too short")
-    _need(qkv.stride(2) == 1, "qkv: a band's elements must be contiguous")
-    _ints(positions, device, 1, "positions")
-    _ints(slots, device, 1, "slots")
-    _need(positions.shape[0] >= rows and slots.shape[0] >= rows, "positions and slots must cover the rows")
+    if width < (heads + 2 * kv_heads) * HEAD_DIM + (heads if wanted else 0):
+        raise ValueError("qkv rows too short")
+    row_stride, band_stride, one = qkv.stride()
+    if one != 1:
+        raise ValueError("qkv: a band's elements must be contiguous")
+    _ints(positions, index, 1, "positions")
+    _ints(slots, index, 1, "slots")
+    if positions.shape[0] < rows or slots.shape[0] < rows:
+        raise ValueError("positions and slots must cover the rows")
+    freqs_ptr = gates_ptr = 0
     if freqs is not None:
-        _need(freqs.dtype == torch.float32 and freqs.device == device and freqs.shape == (HEAD_DIM // 2,)
-              and freqs.is_contiguous(), f"freqs must be 32 float32 on {device}")
-    shape = (rows, bands * heads, HEAD_DIM)
+        if (freqs.dtype is not torch.float32 or freqs.get_device() != index or freqs.shape != (HEAD_DIM // 2,)
+                or not freqs.is_contiguous()):
+            raise ValueError(f"freqs must be 32 float32 on cuda:{index}")
+        freqs_ptr = freqs.data_ptr()
     if q is None:
-        q = torch.empty(shape, dtype=dtype, device=device)
-    if gates is True:
-        gates = torch.empty(shape[:2], dtype=torch.float32, device=device)
-    elif wanted:
-        _need(gates.shape == shape[:2] and gates.dtype == torch.float32 and gates.device == device
-              and gates.is_contiguous(), f"gates must be a contiguous {shape[:2]} float32 tensor on {device}")
+        q = qkv.new_empty((rows, bands * heads, HEAD_DIM))
+    q_stride = _row_stride(q, rows, bands * heads, index, dtype, "q")
+    if wanted:
+        if gates is True:
+            gates = qkv.new_empty((rows, bands * heads), dtype=torch.float32)
+        gates_ptr = _gates_ptr(gates, rows, bands * heads, index)
     else:
         gates = None
-    q_stride = _row_stride(q, shape, device, dtype, "q")
-    status_ptr = _status_ptr(status, device)
+    status_ptr = _status_ptr(status, index)
     if rows:
-        row_stride = qkv.stride(0) if rows > 1 else 0
-        band_stride = qkv.stride(1) if bands > 1 else 0
-        _call(device, "trc_cache_append", _PRECISION[dtype], qkv.data_ptr(), row_stride, band_stride, rows, bands,
-              heads, kv_heads, positions.data_ptr(), slots.data_ptr(), freqs.data_ptr() if freqs is not None else 0,
-              page, n_pages, q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(),
-              gates.data_ptr() if gates is not None else 0, status_ptr)
+        # strides of dimensions of one element say nothing
+        _call(index, "trc_cache_append", _PRECISION[dtype], qkv.data_ptr(), row_stride if rows > 1 else 0,
+              band_stride if bands > 1 else 0, rows, bands, heads, kv_heads, positions.data_ptr(), slots.data_ptr(),
+              freqs_ptr, page, n_pages, q.data_ptr(), q_stride, k_pages.data_ptr(), v_pages.data_ptr(), gates_ptr,
+              status_ptr)
     return q, gates
 
 
-_workspace_bytes: dict[tuple[int, int, int, int], int] = {}  # per device and arguments of trc_cache_workspace
+_workspace_bytes: dict[tuple[int, int, int, int], int] = {}  # by device and arguments of trc_cache_workspace
 
 
 def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -184,42 +200,44 @@ def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     zero for a frame that sees nothing. ``max_new`` / ``max_total``: the longest new part and total as far as the
     host knows; they choose the kernel variant only. ``out``: where to write; otherwise a new tensor, undefined in
     rows behind the last sequence's."""
-    device, dtype = q.device, q.dtype
-    _need(q.is_cuda and q.ndim == 3 and dtype in _PRECISION, "q must be a (rows, heads, 64) fp16 or bf16 CUDA tensor")
-    rows, heads, _ = shape = tuple(q.shape)
-    n_pages, kv_heads, page = _pools(k_pages, v_pages, device, dtype)
-    _need(heads >= 1 and shape[2] == HEAD_DIM and heads % kv_heads == 0, "the cache heads must divide q's heads")
-    _ints(table, device, 2, "table")
-    _ints(cu, device, 1, "cu")
-    _ints(total, device, 1, "total")
-    n = total.shape[0]
-    _need(table.shape[0] == n and cu.shape[0] == n + 1, "table, cu and total must agree in the number of sequences")
-    q_stride = _row_stride(q, shape, device, dtype, "q")
+    dtype = q.dtype
+    if not q.is_cuda or q.ndim != 3 or dtype not in _PRECISION:
+        raise ValueError("q must be a (rows, heads, 64) fp16 or bf16 CUDA tensor")
+    index = q.get_device()
+    rows, heads, dim = q.shape
+    n_pages, kv_heads, page = _pools(k_pages, v_pages, index, dtype)
+    if dim != HEAD_DIM or heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("q must have 64 elements per head, and the cache heads must divide its heads")
+    _ints(table, index, 2, "table")
+    _ints(cu, index, 1, "cu")
+    _ints(total, index, 1, "total")
+    n, columns = table.shape
+    if total.shape[0] != n or cu.shape[0] != n + 1:
+        raise ValueError("table, cu and total must agree in the number of sequences")
+    q_stride = _row_stride(q, rows, heads, index, dtype, "q")
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-    out_stride = _row_stride(out, shape, device, dtype, "out")
-    gates_ptr = 0
-    if gates is not None:
-        _need(gates.shape == shape[:2] and gates.dtype == torch.float32 and gates.device == device
-              and gates.is_contiguous(), f"gates must be a contiguous {shape[:2]} float32 tensor on {device}")
-        gates_ptr = gates.data_ptr()
-    status_ptr = _status_ptr(status, device)
+        out = q.new_empty((rows, heads, HEAD_DIM))
+    out_stride = _row_stride(out, rows, heads, index, dtype, "out")
+    gates_ptr = _gates_ptr(gates, rows, heads, index) if gates is not None else 0
+    status_ptr = _status_ptr(status, index)
     if not rows:
         return out
-    workspace, size = 0, 0
-    if max_total > 512:  # as trc_cache_attention documents
-        key = (device.index, max_new, heads, kv_heads)
+    workspace = size = 0
+    if max_total > MAX_WHOLE:
+        key = (index, max_new, heads, kv_heads)
         size = _workspace_bytes.get(key, 0)
         if not size:
-            with torch.cuda.device(device):
+            with torch.cuda.device(index):
                 size = _lib.load().trc_cache_workspace(max_new, heads, kv_heads)
             if size < 0:
                 _lib.check(size)
+            if len(_workspace_bytes) > 4096:
+                _workspace_bytes.clear()
             _workspace_bytes[key] = size
-        held = torch.empty(size, dtype=torch.uint8, device=device)  # from the current stream's pool
+        held = q.new_empty(size, dtype=torch.uint8)  # of the current stream's pool: free for later work on it
         workspace = held.data_ptr()
-    _call(device, "trc_cache_attention", _PRECISION[dtype], q.data_ptr(), q_stride, k_pages.data_ptr(),
-          v_pages.data_ptr(), table.data_ptr(), table.shape[1], cu.data_ptr(), total.data_ptr(), n, rows, max_new,
-          max_total, heads, kv_heads, page, n_pages, int(causal), window, scale, gates_ptr, out.data_ptr(), out_stride,
+    _call(index, "trc_cache_attention", _PRECISION[dtype], q.data_ptr(), q_stride, k_pages.data_ptr(),
+          v_pages.data_ptr(), table.data_ptr(), columns, cu.data_ptr(), total.data_ptr(), n, rows, max_new, max_total,
+          heads, kv_heads, page, n_pages, 1 if causal else 0, window, scale, gates_ptr, out.data_ptr(), out_stride,
           workspace, size, status_ptr)
     return out
