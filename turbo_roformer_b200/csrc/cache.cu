@@ -14,7 +14,7 @@
 
 #include "../../include/trcuda.h"
 #include "cache_attention.cuh"
-#include "cache_attention_long.cuh"
+#include "cache_attention_tiles.cuh"
 #include "cache_sched.cuh"
 #include "internal.h"
 
@@ -24,14 +24,28 @@ static_assert(kCacheMaxSeqs == TRC_CACHE_MAX_SEQS && kCacheMaxGroup == TRC_CACHE
 
 namespace {
 
-int launched(const char* what, int kernels) {
-  const cudaError_t e = cudaGetLastError();
+// Launches with programmatic dependence on the kernel in front (every kernel of this file waits on the device before
+// it touches memory) and counts the launch.
+template <typename... Params, typename... Args>
+int launch(const char* what, void (*kern)(Params...), dim3 grid, int threads, int smem, cudaStream_t st,
+           const Args&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, Params(args)...);
   if (e != cudaSuccess) {
     char buf[160];
     snprintf(buf, sizeof(buf), "%s launch failed: %s", what, cudaGetErrorString(e));
     return set_last_error(TRC_E_CUDA, buf);
   }
-  count_launches(kernels);
+  count_launches(1);
   return TRC_OK;
 }
 
@@ -82,6 +96,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
   __shared__ int64_t part[2][kPlanThreads / 32];
   __shared__ int flags;
   if (threadIdx.x == 0) flags = 0;
+  grid_wait();
+  grid_release();
   const int per = (a.n_seqs + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
   int64_t rows = 0, pages = 0;
@@ -238,6 +254,8 @@ struct Vec8<__nv_bfloat16> {
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ float2 turn[kAppendFrames][32];  // (cos, sin) of each frame and pair
+  grid_wait();
+  grid_release();
   const int64_t run0 = (int64_t)blockIdx.x * kAppendRun;
   const int frame0 = (int)(run0 / a.vecs);
   const uint32_t rem0 = (uint32_t)(run0 - (int64_t)frame0 * a.vecs);
@@ -337,11 +355,37 @@ int sm_count() {
   return n;
 }
 
-// Rows of a tile: the least of the kernel's variants that holds `rows`, 128 at most.
-int tile_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Which kernel takes a sequence, by its rows per cache head (new frames x query heads that share it). Measured with
+// 496 heads over 1,700 frames (us; HBM floor 34-43 us):
+//   rows                        16   20   28   40   64  128  200  256  384
+//   cache_rows_kernel           ROWS_FIGURES
+//   cache_tiles_kernel          SEPARATE_FIGURES
+//   cache_tiles_kernel, shared  SHARED_FIGURES
+constexpr int kFewRows = 32;      // cache_rows_kernel
+constexpr int kSeparateRows = 256;  // cache_tiles_kernel with separate tiles; above it with shared ones
+constexpr int kCtasPerSm = 2;     // of cache_rows_kernel
 
-constexpr int kCtasPerSm = 2;
-constexpr int kLongRows = 128;  // rows per (sequence, cache head) above which the tcgen05 kernel takes a sequence
+// The launches of a call and where their parts go in the workspace.
+struct Layout {
+  int rows;            // of cache_rows_kernel's tiles
+  int workers;         // its warps
+  bool tiles, shared;  // whether cache_tiles_kernel follows, and how
+  int workers2, rows2;
+  int64_t floats, floats2;  // workspace of the two
+};
+Layout layout_of(int max_new, int group, int sms) {
+  const int64_t most = (int64_t)(max_new > 0 ? max_new : 1) * group;
+  Layout l;
+  l.rows = most <= 16 ? 16 : kFewRows;
+  l.workers = kCtasPerSm * sms * kCrWarps;
+  l.tiles = most > kFewRows;
+  l.shared = most > kSeparateRows;
+  l.workers2 = !l.tiles ? 0 : l.shared ? sms : sms * kCtTiles;
+  l.rows2 = l.shared ? CtSmem<true>::kRows : CtSmem<false>::kRows;
+  l.floats = cache_workspace_floats(l.rows, l.workers);
+  l.floats2 = l.tiles ? cache_workspace_floats(l.rows2, l.workers2) : 0;
+  return l;
+}
 
 // Dynamic shared-memory opt-in, once per kernel and device (`done`: one object per kernel).
 template <typename Kern>
@@ -356,83 +400,85 @@ int allow_smem(Kern kern, int bytes, std::atomic<unsigned long long>& done) {
   return e == cudaSuccess ? TRC_OK : set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
 }
 
-template <typename T>
-int launch_join(const CacheAttnArgs& a, int rows, int ctas, cudaStream_t st) {
-  if (!a.split) return TRC_OK;
-  cache_join_kernel<T><<<dim3(ctas, rows > 32 ? 4 : 1), 256, 0, st>>>(a, rows);
-  return launched("cache attention join", 1);
+template <typename T, int MT>
+int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int workers, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  const int rc = allow_smem(cache_rows_kernel<T, MT>, CrSmem::bytes(kCacheMaxSeqs), done);
+  if (rc) return rc;
+  return launch("cache attention", cache_rows_kernel<T, MT>, dim3(workers / kCrWarps), 32 * kCrWarps,
+                CrSmem::bytes(a.n_seqs), st, mk, mv, a);
 }
 
-template <typename T, int MT, int WM, int WK, int KT, int ST>
-int launch_rows(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int ctas, cudaStream_t st) {
-  using S = CacheRowsSmem<MT, WM, WK, KT, ST>;
-  auto kern = cache_rows_kernel<T, MT, WM, WK, KT, ST>;
-  static std::atomic<unsigned long long> done{0};
-  int rc = allow_smem(kern, S::bytes(kCacheMaxSeqs), done);
-  if (rc) return rc;
-  kern<<<ctas, 32 * WM * WK, S::bytes(a.n_seqs), st>>>(mk, mv, a);
-  rc = launched("cache attention", 1);
-  return rc ? rc : launch_join<T>(a, 16 * MT * WM, ctas, st);
-}
-
-// The tcgen05 kernel moves registers between its warpgroups (setmaxnreg): the split must fit in what the launch gives
-// the block, or the softmax warps' increase would never be granted.
-template <typename T>
-int launch_long(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int ctas, cudaStream_t st) {
-  auto kern = cache_long_kernel<T>;
-  static std::atomic<unsigned long long> done{0};
-  int rc = allow_smem(kern, ClSmem::bytes(kCacheMaxSeqs), done);
-  if (rc) return rc;
-  static std::atomic<int> regs{0};
+// The tcgen05 kernels move registers between their warpgroups (setmaxnreg): the split must fit in what the launch
+// gives the block, or the softmax warps' increase would never be granted.
+template <typename Kern>
+int check_registers(Kern kern, int threads, int wanted, std::atomic<int>& regs) {
   if (regs.load() == 0) {
     cudaFuncAttributes fa;
     const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess) return set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
     regs.store(fa.numRegs);
   }
-  if (4 * 32 * kTaRegsLow + 12 * 32 * kTaRegsHigh > kTaThreads * regs.load())
-    return set_last_error(TRC_E_CUDA, "cache attention: register split larger than the launch's registers");
-  CUtensorMap mq;
+  return wanted > threads * regs.load()
+             ? set_last_error(TRC_E_CUDA, "cache attention: register split larger than the launch's registers")
+             : TRC_OK;
+}
+
+// Q as (64, heads, rows): boxes of a cache head's query heads for the frames of a tile.
+template <typename T>
+int map_q(const CacheAttnArgs& a, CUtensorMap& mq) {
   const uint64_t dims[3] = {64, (uint64_t)a.hq, (uint64_t)a.n_tokens};
   const uint64_t strides[2] = {128, 2 * (uint64_t)(a.n_tokens > 1 ? a.q_stride : (int64_t)a.hq * 64)};
   const uint32_t box[3] = {64, (uint32_t)a.group, (uint32_t)(128 / a.group)};
-  if ((rc = make_tensor_map(&mq, OperandType<T>::kFormat, a.q, 3, dims, strides, box))) return rc;
-  kern<<<ctas, kTaThreads, ClSmem::bytes(a.n_seqs), st>>>(mq, mk, mv, a);
-  rc = launched("cache attention", 1);
-  return rc ? rc : launch_join<T>(a, kClRows, ctas, st);
+  return make_tensor_map(&mq, OperandType<T>::kFormat, a.q, 3, dims, strides, box);
+}
+
+template <typename T, bool SHARED>
+int launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const CacheAttnArgs& a, int sms, cudaStream_t st) {
+  using S = CtSmem<SHARED>;
+  auto kern = cache_tiles_kernel<T, SHARED>;
+  static std::atomic<unsigned long long> done{0};
+  static std::atomic<int> regs{0};
+  CUtensorMap mq;
+  int rc = allow_smem(kern, S::bytes(kCacheMaxSeqs), done);
+  if (!rc) rc = check_registers(kern, S::kThreads, S::kRegs, regs);
+  if (!rc) rc = map_q<T>(a, mq);
+  return rc ? rc
+            : launch("cache attention (tiles)", kern, dim3(sms), S::kThreads, S::bytes(a.n_seqs), st, mq, mk, mv, a);
 }
 
 template <typename T>
-int launch_cache_attention(int64_t most_rows, int page, const void* k, const void* v, CacheAttnArgs a, int sms,
+int launch_cache_attention(const Layout& l, int page, const void* k, const void* v, CacheAttnArgs a, int sms,
                            cudaStream_t st) {
   const int prec = OperandType<T>::kFormat;
   const uint64_t dims[2] = {64, (uint64_t)a.n_pages * a.hkv * page};
   const uint64_t strides[1] = {128};
-  auto maps = [&](uint32_t keys, CUtensorMap& mk, CUtensorMap& mv) {
-    const uint32_t box[2] = {64, (uint32_t)page < keys ? (uint32_t)page : keys};
+  auto maps = [&](int keys, CUtensorMap& mk, CUtensorMap& mv) {
+    const uint32_t box[2] = {64, (uint32_t)(page < keys ? page : keys)};
     const int rc = make_tensor_map(&mk, prec, k, 2, dims, strides, box);
     return rc ? rc : make_tensor_map(&mv, prec, v, 2, dims, strides, box);
   };
   CUtensorMap mk, mv;
-  int rc;
-  const int ctas = kCtasPerSm * sms;
-  if (most_rows > kLongRows) {
-    if ((rc = maps(64, mk, mv))) return rc;
-    a.rows_above = kLongRows;
-    if ((rc = launch_long<T>(mk, mv, a, sms, st))) return rc;
-    a.rows_above = 0;
-    a.rows_upto = kLongRows;
-    return launch_rows<T, 2, 4, 1, 64, 6>(mk, mv, a, ctas, st);
+  int rc = maps(kCrKeys, mk, mv);
+  if (rc) return rc;
+  float* const ws2 = a.ws ? a.ws + l.floats : nullptr;
+  a.rows_above = 0;
+  a.rows_upto = l.tiles ? kFewRows : INT_MAX;
+  rc = l.rows == 16 ? launch_rows<T, 1>(mk, mv, a, l.workers, st) : launch_rows<T, 2>(mk, mv, a, l.workers, st);
+  if (rc) return rc;
+  if (l.tiles) {
+    CacheAttnArgs b = a;
+    b.rows_above = kFewRows;
+    b.rows_upto = INT_MAX;
+    b.ws = ws2;
+    if ((rc = maps(kCacheStep, mk, mv))) return rc;
+    rc = l.shared ? launch_tiles<T, true>(mk, mv, b, sms, st) : launch_tiles<T, false>(mk, mv, b, sms, st);
+    if (rc) return rc;
   }
-  const int rows = tile_rows(most_rows);
-  if ((rc = maps(rows <= 16 ? 32 : 64, mk, mv))) return rc;
-  // stages: 96 KB per CTA, two CTAs per SM
-  switch (rows) {
-    case 16: return launch_rows<T, 1, 1, 4, 32, 3>(mk, mv, a, ctas, st);
-    case 32: return launch_rows<T, 1, 2, 2, 64, 3>(mk, mv, a, ctas, st);
-    case 64: return launch_rows<T, 1, 4, 1, 64, 6>(mk, mv, a, ctas, st);
-    default: return launch_rows<T, 2, 4, 1, 64, 6>(mk, mv, a, ctas, st);
-  }
+  if (!a.split) return TRC_OK;
+  const CacheJoin j = {l.workers, l.rows, l.rows2, ws2};
+  return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + l.workers2, l.tiles ? 4 : 1), 256, 0, st,
+                a, j);
 }
 
 }  // namespace
@@ -484,8 +530,8 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
   // blocks for the rows; the fresh pages are at most as many plus one per sequence
   const int64_t most = (int64_t)max_rows + n_seqs;
   const int blocks = (int)((most + trc::kPlanThreads - 1) / trc::kPlanThreads);
-  trc::cache_plan_kernel<<<blocks < 2 * sms ? blocks : 2 * sms, trc::kPlanThreads, smem, (cudaStream_t)stream>>>(a);
-  return trc::launched("cache plan", 1);
+  return trc::launch("cache plan", trc::cache_plan_kernel, dim3(blocks < 2 * sms ? blocks : 2 * sms), trc::kPlanThreads,
+                     smem, (cudaStream_t)stream, a);
 }
 
 int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64_t band_stride, int n_rows, int bands,
@@ -539,11 +585,8 @@ int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64
   const int64_t blocks = ((int64_t)n_rows * vecs + trc::kAppendRun - 1) / trc::kAppendRun;
   if (blocks > INT_MAX) return set_last_error(TRC_E_INVALID, "cache append: too many rows");
   cudaStream_t st = (cudaStream_t)stream;
-  if (precision == TRC_PREC_FP16)
-    trc::cache_append_kernel<__half><<<(unsigned)blocks, trc::kAppendThreads, 0, st>>>(a);
-  else
-    trc::cache_append_kernel<__nv_bfloat16><<<(unsigned)blocks, trc::kAppendThreads, 0, st>>>(a);
-  return trc::launched("cache append", 1);
+  auto kern = precision == TRC_PREC_FP16 ? trc::cache_append_kernel<__half> : trc::cache_append_kernel<__nv_bfloat16>;
+  return trc::launch("cache append", kern, dim3((unsigned)blocks), trc::kAppendThreads, 0, st, a);
 }
 
 int64_t trc_cache_workspace(int max_new, int heads, int kv_heads) {
@@ -552,12 +595,8 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads) {
     return set_last_error(TRC_E_INVALID, "cache workspace: bad sizes");
   const int sms = trc::sm_count();
   if (!sms) return set_last_error(TRC_E_CUDA, "cache workspace: no current CUDA device");
-  const int64_t most = (int64_t)(max_new > 0 ? max_new : 1) * (heads / kv_heads);
-  // launches of one call follow one another on its stream and share the workspace
-  int64_t floats = trc::cache_workspace_floats(trc::tile_rows(most), trc::kCtasPerSm * sms);
-  if (most > trc::kLongRows && trc::cache_workspace_floats(trc::kClRows, sms) > floats)
-    floats = trc::cache_workspace_floats(trc::kClRows, sms);
-  return 4 * floats;
+  const trc::Layout l = trc::layout_of(max_new, heads / kv_heads, sms);
+  return 4 * (l.floats + l.floats2);
 }
 
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
@@ -614,20 +653,16 @@ int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const 
   a.causal = causal != 0;
   a.window = window > 1 << 30 ? 0 : window;  // longer than any sequence
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.rows_above = 0;
-  a.rows_upto = INT_MAX;
-  a.min_share = 4;
   a.split = max_total > TRC_CACHE_MAX_WHOLE;
-  const int64_t most = (int64_t)(max_new > 0 ? max_new : 1) * a.group;
-  if (a.split) {
-    if (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 16 ||
-        workspace_bytes < trc_cache_workspace(max_new, heads, kv_heads))
-      return set_last_error(TRC_E_INVALID, "cache attention: workspace missing or smaller than trc_cache_workspace");
-  }
+  a.min_share = a.split ? 2 : 1;  // steps: a part of less than 128 keys costs more to join than it saves
+  const trc::Layout l = trc::layout_of(max_new, a.group, sms);
+  if (a.split && (!d_workspace || reinterpret_cast<uintptr_t>(d_workspace) % 16 ||
+                  workspace_bytes < 4 * (l.floats + l.floats2)))
+    return set_last_error(TRC_E_INVALID, "cache attention: workspace missing or smaller than trc_cache_workspace");
   cudaStream_t st = (cudaStream_t)stream;
   return precision == TRC_PREC_FP16
-             ? trc::launch_cache_attention<__half>(most, page, d_k, d_v, a, sms, st)
-             : trc::launch_cache_attention<__nv_bfloat16>(most, page, d_k, d_v, a, sms, st);
+             ? trc::launch_cache_attention<__half>(l, page, d_k, d_v, a, sms, st)
+             : trc::launch_cache_attention<__nv_bfloat16>(l, page, d_k, d_v, a, sms, st);
 }
 
 }  // extern "C"

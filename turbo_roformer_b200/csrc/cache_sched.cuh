@@ -23,6 +23,17 @@ constexpr int kCacheMaxSeqs = 2048;
 constexpr int kCacheMaxGroup = 64;
 constexpr int kCacheStep = 64;  // keys per step
 
+// Programmatic dependent launch: every kernel here may start before the one in front of it on the stream has ended
+// (its launch and set-up overlap that one's tail), lets its own successor do the same, and waits before it touches
+// global memory.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// a / b for a >= 0, b > 0, the short way where both fit 32 bits
+__device__ __forceinline__ int64_t div_pos(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
 struct CacheAttnArgs {
   const void* q;        // [n_tokens][hq][64] 16-bit, q_stride elements from token to token
   void* out;            // like q, out_stride
@@ -98,7 +109,7 @@ struct CacheItem {
       if (left < all) break;
       left -= all;
     }
-    head = (int)(left / (t1 - t0));
+    head = (int)div_pos(left, t1 - t0);
     start = at - (left - (int64_t)head * (t1 - t0));
   }
   __device__ __forceinline__ void next(const CacheAttnArgs& a, int tpt) {
@@ -120,7 +131,7 @@ struct CacheItem {
 
 // A CTA's share of a line of `length` steps.
 __device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t length, int ctas) {
-  return max((length + ctas - 1) / ctas, (int64_t)a.min_share);
+  return max(div_pos(length + ctas - 1, ctas), (int64_t)a.min_share);
 }
 
 // The line's scan, by all `threads` threads of the CTA: prefix[r] = steps before sequence r, prefix[n_seqs] =
@@ -202,7 +213,7 @@ struct CacheWalk {
   // CTAs that work on this item, when it is begun here and not ended
   __device__ __forceinline__ int parts() const {
     const int64_t w = s1 - s0;  // a share that an item outlasts is not the line's last, so it is a full one
-    return 1 + (int)((it.start + (it.t1 - it.t0) - 1 - s0) / w);
+    return 1 + (int)div_pos(it.start + (it.t1 - it.t0) - 1 - s0, w);
   }
 };
 
