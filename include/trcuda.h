@@ -189,7 +189,7 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
  * NULL: no rotation). d_q [n_rows][bands * heads][64], q_stride elements between frames; k and v go to
  * d_slots[row] of the pools (bands * kv_heads cache heads); d_gates [n_rows][bands * heads] fp32 = sigmoid
  * (NULL: none). Rows of slot < 0 are skipped; a slot behind the pool is not written and sets *d_status. Row
- * starts are multiples of 16 bytes. */
+ * starts and d_freqs are 16-byte aligned; at most 1,048,560 rows, 4,096 bands and 4,096 heads per band. */
 int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64_t band_stride, int n_rows, int bands,
                      int heads, int kv_heads, const int32_t* d_positions, const int32_t* d_slots, const float* d_freqs,
                      int page, int n_pages, void* d_q, int64_t q_stride, void* d_k, void* d_v, float* d_gates,

@@ -42,7 +42,8 @@ def test_plan_refuses(change, word):
     (dict(n_pages=0), "sizes"), (dict(page=256), "page"), (dict(qkv=None), "null"), (dict(slots=None), "null"),
     (dict(k=None), "null"), (dict(row_stride=196), "16-byte"), (dict(q=ctypes.c_void_p(4104)), "16-byte"),
     (dict(bands=2, band_stride=128, q_stride=128), "strides"), (dict(q_stride=56), "strides"),
-    (dict(bands=4096, heads=64, kv_heads=64, band_stride=12288, q_stride=64 * 64 * 4096), "too large")])
+    (dict(freqs=ctypes.c_void_p(4100)), "16-byte"),
+    (dict(rows=1 << 21), "1,048,560"), (dict(rows=1048561), "1,048,560")])
 def test_append_refuses(change, word):
     refused("trc_cache_append", tuple({**APPEND, **change}.values()), word)
 

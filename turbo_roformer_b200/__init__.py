@@ -26,7 +26,8 @@ def __getattr__(name):
     if name in ("CachePlan", "cache_plan", "cache_append", "cache_attention"):
         from . import frame_cache
 
-        return getattr(frame_cache, name)
+        value = globals()[name] = getattr(frame_cache, name)  # found at once from now on: a push's calls are short
+        return value
     if name == "CudaBSRoformer":
         from .backend import CudaBSRoformer
 

@@ -210,16 +210,15 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
 }
 
 // ------------------------------------------------------------------------------------------------ append
-// One thread per 16-byte vector (8 elements = 4 rotary pairs) of the rows, kAppendVecs vectors per thread in
-// flight; HBM bound (each element is read once and written once). A block takes a flat run of vectors, which may
-// span many short rows or a part of a long one; the angles of its frames (position x frequency in fp64, reduced
-// to half turns, because fp32 loses the angle of far positions) are computed once per block and shared by all
-// heads.
+// HBM bound: each element is read once and written once. Eight lanes own a head row (64 elements, 16 bytes = 4 rotary
+// pairs each). A block takes one band of up to 16 consecutive frames, and each thread one frame of it and every
+// 32 / frames-th head row, so that
+//   * its four angles (position x frequency in fp64, reduced to half turns, because fp32 loses the angle of far
+//     positions) are computed once, while its first loads travel, and stay in registers for all its heads;
+//   * the 128-byte rows that a head's frames write to a page lie one behind the other.
 constexpr int kAppendThreads = 256;
-constexpr int kAppendVecs = 4;
-constexpr int kAppendRun = kAppendThreads * kAppendVecs;
-// frames that a run can touch: a frame has at least 24 vectors (one q, k and v head)
-constexpr int kAppendFrames = kAppendRun / 24 + 2;
+constexpr int kAppendFlight = 4;  // head rows per thread in flight
+constexpr int kAppendFrames = 16;
 
 struct AppendArgs {
   const void* qkv;
@@ -232,114 +231,89 @@ struct AppendArgs {
   int* status;
   int n_tokens, bands, heads, kv_heads, page_log2;
   int64_t n_slots;
-  int band_vecs, vecs;        // 16-byte vectors per band and per frame
-  uint32_t band_mul, frame_mul;  // x / d = umulhi(x, mul) for the x that occur (see div_mul)
+  int frames;  // frames of a block: 1, 2, 4, 8 or 16
 };
-
-// umulhi(x, ceil(2^32 / d)) = x / d for x * d < 2^32 (the error x (mul d - 2^32) / (2^32 d) stays below 1 / d)
-uint32_t div_mul(uint32_t d) { return d == 1 ? 0u : (uint32_t)((0x100000000ull + d - 1) / d); }
-__device__ __forceinline__ uint32_t div_by(uint32_t x, uint32_t mul) { return mul ? __umulhi(x, mul) : x; }
 
 template <typename T>
 struct Vec8;
 template <>
 struct Vec8<__half> {
   __device__ static float2 to_f2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+  __device__ static float to_f(__half x) { return __half2float(x); }
 };
 template <>
 struct Vec8<__nv_bfloat16> {
   __device__ static float2 to_f2(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); }
+  __device__ static float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 };
 
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __grid_constant__ AppendArgs a) {
-  __shared__ float2 turn[kAppendFrames][32];  // (cos, sin) of each frame and pair
   grid_wait();
   grid_release();
-  const int64_t run0 = (int64_t)blockIdx.x * kAppendRun;
-  const int frame0 = (int)(run0 / a.vecs);
-  const uint32_t rem0 = (uint32_t)(run0 - (int64_t)frame0 * a.vecs);
-
-  // the run's loads first: the angles are computed while they travel
-  uint4 data[kAppendVecs];
-  int frame[kAppendVecs], band[kAppendVecs], sub[kAppendVecs];
+  const int band = blockIdx.x, tok0 = blockIdx.y * a.frames;
+  const int slot_id = threadIdx.x >> 3, d = (threadIdx.x & 7) * 8;  // of 32 head rows at a time; first element
+  const int f = slot_id & (a.frames - 1), step = 32 / a.frames;
+  const int tok = tok0 + f, rows = a.heads + 2 * a.kv_heads;
+  if (tok >= a.n_tokens) return;
+  const T* band_row = static_cast<const T*>(a.qkv) + tok * a.tok_stride + band * a.band_stride;
+  const T* src = band_row + d;
+  int row = slot_id / a.frames;
+  uint4 data[kAppendFlight];
+  auto load = [&](int r) {
 #pragma unroll
-  for (int i = 0; i < kAppendVecs; ++i) {
-    const uint32_t x = rem0 + i * kAppendThreads + threadIdx.x;
-    const uint32_t f = div_by(x, a.frame_mul);
-    const uint32_t in = x - f * a.vecs;
-    const uint32_t b = div_by(in, a.band_mul);
-    frame[i] = (int)f;
-    band[i] = (int)b;
-    sub[i] = (int)(in - b * a.band_vecs);
-    const int64_t tok = (int64_t)frame0 + f;
-    data[i] = make_uint4(0, 0, 0, 0);
-    if (tok >= a.n_tokens || a.slots[tok] < 0) {
-      frame[i] = -1;  // behind the last row, or a row of padding
-    } else {
-      const T* src = static_cast<const T*>(a.qkv) + tok * a.tok_stride + b * a.band_stride + (int64_t)sub[i] * 8;
-      const int gate0 = (a.heads + 2 * a.kv_heads) * 8;
-      if (sub[i] < gate0 || (sub[i] - gate0) * 8 + 8 <= a.heads) {
-        data[i] = __ldcs(reinterpret_cast<const uint4*>(src));
-      } else {  // the last gates: no reads behind them
-        uint16_t tail[8] = {};
-        for (int e = 0; e < a.heads - (sub[i] - gate0) * 8; ++e) tail[e] = reinterpret_cast<const uint16_t*>(src)[e];
-        data[i] = make_uint4(tail[0] | (uint32_t)tail[1] << 16, tail[2] | (uint32_t)tail[3] << 16,
-                             tail[4] | (uint32_t)tail[5] << 16, tail[6] | (uint32_t)tail[7] << 16);
-      }
-    }
-  }
-  const int frames = (int)div_by(rem0 + kAppendRun - 1, a.frame_mul) + 1;
-  for (int x = threadIdx.x; x < frames * 32; x += kAppendThreads) {
-    const int64_t tok = (int64_t)frame0 + (x >> 5);
-    float2 t = make_float2(1.f, 0.f);
-    if (a.freqs && tok < a.n_tokens) {
+    for (int i = 0; i < kAppendFlight; ++i)
+      if (r + i * step < rows) data[i] = __ldcs(reinterpret_cast<const uint4*>(src + (r + i * step) * 64));
+  };
+  load(row);
+  const int slot = a.slots[tok];
+  if (slot < 0) return;  // a row of padding
+  float2 turn[4] = {{1.f, 0.f}, {1.f, 0.f}, {1.f, 0.f}, {1.f, 0.f}};
+  if (a.freqs) {
+    const double pos = a.positions[tok];
+    const float4 w = *reinterpret_cast<const float4*>(a.freqs + (d >> 1));
+    const float fr[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
       // half turns: the angle over pi, modulo 2; fp64 keeps 1e-9 of a turn at positions past 2^30
-      const double h = (double)a.positions[tok] * (double)a.freqs[x & 31] * 0.31830988618379067154;
-      sincospif((float)(h - 2.0 * rint(0.5 * h)), &t.y, &t.x);
+      const double h = pos * (double)fr[p] * 0.31830988618379067154;
+      sincospif((float)(h - 2.0 * rint(0.5 * h)), &turn[p].y, &turn[p].x);
     }
-    turn[x >> 5][x & 31] = t;
   }
-  __syncthreads();
+  const bool known = slot < a.n_slots;
+  if (!known) record_error(a.status, kErrBadArgs);
+  // where head row r of q, k and v goes: the cache's rows are a page apart
+  const int64_t page_row = ((((int64_t)(slot >> a.page_log2) * a.bands + band) * a.kv_heads) << a.page_log2) +
+                           (slot & ((1 << a.page_log2) - 1));
+  T* const q = static_cast<T*>(a.q) + tok * a.q_stride + (int64_t)band * a.heads * 64 + d;
+  T* const k = static_cast<T*>(a.k) + page_row * 64 + d - ((int64_t)a.heads << (a.page_log2 + 6));
+  T* const v = static_cast<T*>(a.v) + page_row * 64 + d - ((int64_t)(a.heads + a.kv_heads) << (a.page_log2 + 6));
+  for (; row < rows; row += kAppendFlight * step) {
 #pragma unroll
-  for (int i = 0; i < kAppendVecs; ++i) {
-    if (frame[i] < 0) continue;
-    const int64_t tok = (int64_t)frame0 + frame[i];
-    const int head = sub[i] >> 3, d = (sub[i] & 7) * 8;
-    uint32_t u[4] = {data[i].x, data[i].y, data[i].z, data[i].w};
-    if (head < a.heads + a.kv_heads && a.freqs) {
+    for (int i = 0; i < kAppendFlight; ++i) {
+      const int r = row + i * step;
+      if (r >= rows) break;
+      uint4 u = data[i];
+      if (r < a.heads + a.kv_heads && a.freqs) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float2 x = Vec8<T>::to_f2(u[p]), t = turn[frame[i]][(d >> 1) + p];
-        u[p] = OperandType<T>::pack2(x.x * t.x - x.y * t.y, x.y * t.x + x.x * t.y);
+        for (int p = 0; p < 4; ++p) {
+          const float2 y = Vec8<T>::to_f2(w[p]), t = turn[p];
+          w[p] = OperandType<T>::pack2(y.x * t.x - y.y * t.y, y.y * t.x + y.x * t.y);
+        }
       }
+      if (r < a.heads)
+        *reinterpret_cast<uint4*>(q + r * 64) = u;
+      else if (known)
+        *reinterpret_cast<uint4*>((r < a.heads + a.kv_heads ? k : v) + ((int64_t)r << (a.page_log2 + 6))) = u;
     }
-    const uint4 out = make_uint4(u[0], u[1], u[2], u[3]);
-    if (head < a.heads) {
-      T* dst = static_cast<T*>(a.q) + tok * a.q_stride + ((int64_t)band[i] * a.heads + head) * 64 + d;
-      *reinterpret_cast<uint4*>(dst) = out;
-    } else if (head < a.heads + 2 * a.kv_heads) {
-      const int64_t slot = a.slots[tok];
-      if (slot >= a.n_slots) {
-        record_error(a.status, kErrBadArgs);
-        continue;
-      }
-      const bool is_v = head >= a.heads + a.kv_heads;
-      const int64_t kvh = (int64_t)band[i] * a.kv_heads + head - a.heads - (is_v ? a.kv_heads : 0);
-      const int64_t page = slot >> a.page_log2, in_page = slot & ((1 << a.page_log2) - 1);
-      T* dst = static_cast<T*>(is_v ? a.v : a.k) +
-               ((((page * a.bands * a.kv_heads + kvh) << a.page_log2) + in_page) * 64 + d);
-      *reinterpret_cast<uint4*>(dst) = out;
-    } else {
-      const int h0 = (sub[i] - (a.heads + 2 * a.kv_heads) * 8) * 8;
-      float* dst = a.gates + (tok * a.bands + band[i]) * a.heads + h0;
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float2 x = Vec8<T>::to_f2(u[p]);
-        if (h0 + 2 * p < a.heads) dst[2 * p] = 1.0f / (1.0f + expf(-x.x));
-        if (h0 + 2 * p + 1 < a.heads) dst[2 * p + 1] = 1.0f / (1.0f + expf(-x.y));
-      }
-    }
+    if (row + kAppendFlight * step < rows) load(row + kAppendFlight * step);
+  }
+  if (a.gates) {
+    const T* logits = band_row + rows * 64;
+    float* g = a.gates + ((int64_t)tok * a.bands + band) * a.heads;
+    for (int h = slot_id / a.frames * 8 + (threadIdx.x & 7); h < a.heads; h += step * 8)
+      g[h] = 1.0f / (1.0f + expf(-Vec8<T>::to_f(logits[h])));
   }
 }
 
@@ -477,7 +451,7 @@ int launch_cache_attention(const Layout& l, int page, const void* k, const void*
   }
   if (!a.split) return TRC_OK;
   const CacheJoin j = {l.workers, l.rows, l.rows2, ws2};
-  return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + l.workers2, l.tiles ? 4 : 1), 256, 0, st,
+  return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + 4 * l.workers2), 256, 0, st,
                 a, j);
 }
 
@@ -551,8 +525,8 @@ int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64
   const int64_t width = (int64_t)(heads + 2 * kv_heads) * 64 + (d_gates ? heads : 0);
   if (row_stride % 8 || band_stride % 8 || q_stride % 8 || reinterpret_cast<uintptr_t>(d_qkv) % 16 ||
       reinterpret_cast<uintptr_t>(d_q) % 16 || reinterpret_cast<uintptr_t>(d_k) % 16 ||
-      reinterpret_cast<uintptr_t>(d_v) % 16)
-    return set_last_error(TRC_E_INVALID, "cache append: rows must start on 16-byte boundaries");
+      reinterpret_cast<uintptr_t>(d_v) % 16 || reinterpret_cast<uintptr_t>(d_freqs) % 16)
+    return set_last_error(TRC_E_INVALID, "cache append: rows (and d_freqs) must start on 16-byte boundaries");
   if ((bands > 1 && band_stride < width) || (n_rows > 1 && q_stride < (int64_t)bands * heads * 64))
     return set_last_error(TRC_E_INVALID, "cache append: strides shorter than the rows");
   trc::AppendArgs a;
@@ -574,19 +548,17 @@ int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64
   a.kv_heads = kv_heads;
   a.page_log2 = lp;
   a.n_slots = (int64_t)n_pages << lp;
-  a.band_vecs = (heads + 2 * kv_heads) * 8 + (d_gates ? (heads + 7) / 8 : 0);
-  const int64_t vecs = (int64_t)bands * a.band_vecs;
-  // div_mul's range: an index below vecs + a run, times the divisor
-  if ((vecs + trc::kAppendRun) * vecs >= (int64_t)1 << 32)
-    return set_last_error(TRC_E_INVALID, "cache append: bands x heads too large");
-  a.vecs = (int)vecs;
-  a.band_mul = trc::div_mul((uint32_t)a.band_vecs);
-  a.frame_mul = trc::div_mul((uint32_t)vecs);
-  const int64_t blocks = ((int64_t)n_rows * vecs + trc::kAppendRun - 1) / trc::kAppendRun;
-  if (blocks > INT_MAX) return set_last_error(TRC_E_INVALID, "cache append: too many rows");
+  if (n_rows > 1 << 20 || (n_rows + trc::kAppendFrames - 1) / trc::kAppendFrames > 65535)  // the grid's second axis
+    return set_last_error(TRC_E_INVALID, "cache append: more than 1,048,560 rows");
+  const int sms = trc::sm_count();
+  if (!sms) return set_last_error(TRC_E_CUDA, "cache append: no current CUDA device");
+  // the most frames per block that leave eight blocks per SM
+  a.frames = trc::kAppendFrames;
+  while (a.frames > 1 && (int64_t)((n_rows + a.frames - 1) / a.frames) * bands < 8ll * sms) a.frames /= 2;
   cudaStream_t st = (cudaStream_t)stream;
   auto kern = precision == TRC_PREC_FP16 ? trc::cache_append_kernel<__half> : trc::cache_append_kernel<__nv_bfloat16>;
-  return trc::launch("cache append", kern, dim3((unsigned)blocks), trc::kAppendThreads, 0, st, a);
+  return trc::launch("cache append", kern, dim3(bands, (n_rows + a.frames - 1) / a.frames), trc::kAppendThreads, 0, st,
+                     a);
 }
 
 int64_t trc_cache_workspace(int max_new, int heads, int kv_heads) {

@@ -96,6 +96,9 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
   }
   grid_wait();
   grid_release();
+  // the first table lines travel while the lengths are read
+  if ((int64_t)threadIdx.x * 32 < (int64_t)args.n_seqs * args.table_stride)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(args.table + threadIdx.x * 32));
   const int tpt = kRows / args.group;
   // its barriers cover the initialisation above
   const int workers = gridDim.x * kCrWarps, worker = warp * gridDim.x + blockIdx.x;
@@ -383,8 +386,8 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
 }
 
 // Joins the parts of items that were divided among workers, for one launch's workers (0 .. workers - 1) and, behind
-// them, a second launch's with a workspace of its own. Blocks (w, y) take the item that worker w began and did not
-// end, if there is one. A warp takes a row at a time and reads two parts at once (16 lanes x 4 dims each); where an item
+// them, a second launch's with a workspace of its own. A block takes the item that its worker began and did not end, if
+// there is one (four share the rows of one of the second launch's). A warp takes a row at a time and reads two parts at once (16 lanes x 4 dims each); where an item
 // has few rows in many parts, 2, 4 or 8 warps share a row and meet in shared memory.
 struct CacheJoin {
   int workers, rows;  // of the first launch; rows of its slots
@@ -410,10 +413,12 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
   grid_wait();
   grid_release();
   CacheAttnArgs args = first;
-  int worker = blockIdx.x, workers = j.workers, tile_rows = j.rows;
-  if (worker >= j.workers) {
-    worker -= j.workers;
-    workers = gridDim.x - j.workers;
+  int worker = blockIdx.x, workers = j.workers, tile_rows = j.rows, y = 0, ny = 1;
+  if (worker >= j.workers) {  // four blocks per worker of the second launch
+    y = (worker - j.workers) & 3;
+    ny = 4;
+    worker = (worker - j.workers) >> 2;
+    workers = ((int)gridDim.x - j.workers) >> 2;
     tile_rows = j.rows2;
     args.ws = j.ws2;
   }
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane >> 4, d = (lane & 15) * 4;
   const int per = 8 / share;  // rows of a block at a time
-  for (int row0 = blockIdx.y * per; row0 < rows; row0 += gridDim.y * per) {
+  for (int row0 = y * per; row0 < rows; row0 += ny * per) {
     const int row = row0 + warp / share;
     JoinSum s = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
     if (row < rows) {

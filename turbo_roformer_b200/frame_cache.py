@@ -117,7 +117,7 @@ def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, fre
         raise ValueError("max_rows out of range")
     sizes = (n + 1, n, max_rows, max_rows, 2)
     if out is None:
-        out = CachePlan(*cached.new_empty(sum(sizes)).split_with_sizes(sizes))  # one allocation
+        out = CachePlan._make(cached.new_empty(2 * (n + max_rows) + 3).split_with_sizes(sizes))  # one allocation
     else:
         for t, size, name in zip(out, sizes, CachePlan._fields):
             _ints(t, index, 1, name)
