@@ -436,6 +436,7 @@ int launch_cache_attention(const Layout& l, int page, const void* k, const void*
   int rc = maps(kCrKeys, mk, mv);
   if (rc) return rc;
   float* const ws2 = a.ws ? a.ws + l.floats : nullptr;
+  a.whole_from = 16;
   a.rows_above = 0;
   a.rows_upto = l.tiles ? kFewRows : INT_MAX;
   rc = l.rows == 16 ? launch_rows<T, 1>(mk, mv, a, l.workers, st) : launch_rows<T, 2>(mk, mv, a, l.workers, st);
@@ -444,6 +445,7 @@ int launch_cache_attention(const Layout& l, int page, const void* k, const void*
     CacheAttnArgs b = a;
     b.rows_above = kFewRows;
     b.rows_upto = INT_MAX;
+    b.whole_from = 6;  // a divided tile leaves 34 KB or more in the workspace
     b.ws = ws2;
     if ((rc = maps(kCacheStep, mk, mv))) return rc;
     rc = l.shared ? launch_tiles<T, true>(mk, mv, b, sms, st) : launch_tiles<T, false>(mk, mv, b, sms, st);
@@ -451,7 +453,7 @@ int launch_cache_attention(const Layout& l, int page, const void* k, const void*
   }
   if (!a.split) return TRC_OK;
   const CacheJoin j = {l.workers, l.rows, l.rows2, ws2};
-  return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + 4 * l.workers2), 256, 0, st,
+  return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + kJoinBlocks * l.workers2), 256, 0, st,
                 a, j);
 }
 

@@ -387,8 +387,9 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
 
 // Joins the parts of items that were divided among workers, for one launch's workers (0 .. workers - 1) and, behind
 // them, a second launch's with a workspace of its own. A block takes the item that its worker began and did not end, if
-// there is one (four share the rows of one of the second launch's). A warp takes a row at a time and reads two parts at once (16 lanes x 4 dims each); where an item
+// there is one (kJoinBlocks of them share the rows of one of the second launch's). A warp takes a row at a time and reads two parts at once (16 lanes x 4 dims each); where an item
 // has few rows in many parts, 2, 4 or 8 warps share a row and meet in shared memory.
+constexpr int kJoinBlocks = 8;
 struct CacheJoin {
   int workers, rows;  // of the first launch; rows of its slots
   int rows2;
@@ -414,11 +415,11 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
   grid_release();
   CacheAttnArgs args = first;
   int worker = blockIdx.x, workers = j.workers, tile_rows = j.rows, y = 0, ny = 1;
-  if (worker >= j.workers) {  // four blocks per worker of the second launch
-    y = (worker - j.workers) & 3;
-    ny = 4;
-    worker = (worker - j.workers) >> 2;
-    workers = ((int)gridDim.x - j.workers) >> 2;
+  if (worker >= j.workers) {  // kJoinBlocks per worker of the second launch
+    ny = kJoinBlocks;
+    y = (worker - j.workers) % ny;
+    worker = (worker - j.workers) / ny;
+    workers = ((int)gridDim.x - j.workers) / ny;
     tile_rows = j.rows2;
     args.ws = j.ws2;
   }

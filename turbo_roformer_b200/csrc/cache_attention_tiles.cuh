@@ -15,8 +15,8 @@
 //     more (the tensor pipe is shared by the three), and a step lasts about 2,600. Keys and values have stages of
 //     their own, K freed by S, V by P V.
 //   * V rows outside the item's keys (behind the sequence's end, before the window) are zeroed in shared memory by the
-//     softmax warps before they hand on P, because pages hold anything there and 0 x NaN is NaN (tiles that share the
-//     stage all write the same zeros, each before its own product); scores are replaced per row.
+//     producer before it hands the stage on, because pages hold anything there and 0 x NaN is NaN; scores are replaced
+//     per row, behind one vote per step.
 //   * A run that is not a whole item leaves its rows' sums, maxima and weights in the workspace for the join.
 // Roles: warps 0-2 MMA issuers of tiles 0-2, warp 3 owns TMEM, producers, softmax + epilogue (CtSmem).
 #pragma once
@@ -36,6 +36,8 @@ struct CacheRun {
   int head;         // cache head; -1: no more runs
   int slot;         // workspace slot, -1 for a whole item
   int lo, hi;       // keys that some row sees
+  int seq;          // sequence
+  int unused;
 };
 
 template <bool SHARED>
@@ -51,7 +53,8 @@ struct CtSmem {
   static constexpr int kKV = kQ + kQBufs * kCtTiles * kTileQ;                                    // [channels][K, V][stages]
   static constexpr int kScale = kKV + kChannels * 2 * kStages * kTileKV;                // [tiles][128] fp32
   static constexpr int kRun = kScale + kCtTiles * 128 * 4;                              // [channels][kCtRuns]
-  static constexpr int kBar = kRun + kChannels * kCtRuns * (int)sizeof(CacheRun);
+  static constexpr int kWalk = kRun + kChannels * kCtRuns * (int)sizeof(CacheRun);      // [channels] CacheWalk
+  static constexpr int kBar = kWalk + kChannels * 128;
   static constexpr int kScan = kBar + 768 + 256;
   static constexpr int bytes(int n_seqs) { return kScan + (n_seqs + 1) * 8 + 1024; }
   // Warps 0-2 issue; the producers are warp 3 (shared) or warps 4-6; then twelve softmax warps. Registers per thread
@@ -64,6 +67,7 @@ struct CtSmem {
   static constexpr int kRegsLoad = 56;
   static constexpr int kRegsSoftmax = SHARED ? 152 : 128;
   static constexpr int kRegs = 128 * (kRegsIssue + (SHARED ? 0 : kRegsLoad) + 3 * kRegsSoftmax);
+  static_assert(kBar % 8 == 0 && kScan % 8 == 0, "alignment");
   static_assert(kScan + (kCacheMaxSeqs + 1) * 8 + 1024 <= 232448, "shared memory per CTA");
 };
 
@@ -88,7 +92,8 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
   uint64_t* p_free = p_full + kCtTiles;
   uint64_t* o_free = p_free + kCtTiles;
   uint64_t* drain = o_free + kCtTiles;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + kCtTiles);
+  uint64_t* raw = drain + kCtTiles;            // [channels] values that are still to be zeroed in part
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw + kCh);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int64_t* part = reinterpret_cast<int64_t*>(smem + S::kBar + 768);
   int64_t* prefix = reinterpret_cast<int64_t*>(smem + S::kScan);
@@ -101,6 +106,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
   if (threadIdx.x == 0) {
     for (int c = 0; c < kCh * kBufs; ++c) {
       mbar_init(&q_full[c], 1);
+      if (c < kCh) mbar_init(&raw[c], 1);
       mbar_init(&q_empty[c], 5 * S::kTilesPer);  // a tile's issuer, and its softmax warps once they have the run
     }
     for (int s = 0; s < kCh * kStages; ++s) {
@@ -251,48 +257,79 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       uint8_t* v_ring = k_ring + kStages * S::kTileKV;
       const int page = 1 << args.page_log2, box = min(page, kCacheStep), boxes = kCacheStep / box;
       const int nowhere = (args.n_pages * args.hkv) << args.page_log2;  // behind the pool: TMA's zero fill
-      CacheWalk w;
-      w.begin(args, tpt, prefix, worker, workers, split);
-      if (args.split && lane == 0) cache_record(args, worker)->parts = 0;
+      // the walk lives in shared memory, lane 0's: it takes more registers than the loads have to spare
+      CacheWalk& w = *reinterpret_cast<CacheWalk*>(smem + S::kWalk + c * 128);
+      static_assert(sizeof(CacheWalk) <= 128, "layout");
+      if (lane == 0) {
+        w.begin(args, tpt, prefix, worker, workers, split);
+        if (args.split) cache_record(args, worker)->parts = 0;
+      }
       bool ok = true;
       int k_count = 0, v_count = 0, r = 0;
-      auto request = [&](const CUtensorMap& map, uint8_t* ring, uint64_t* full, uint64_t* empty, int& count, int y) {
-        const int st = count % kStages;
-        const uint32_t use = (uint32_t)(count / kStages);
-        if (ok) ok = mbar_wait_warp(&empty[st], (use & 1) ^ 1, args.status, kErrWaitProducer, abort_flag);
-        if (!ok) return;
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], S::kTileKV);
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = mbar_wait_warp(bar, parity, args.status, kErrWaitProducer, abort_flag);
+        return ok;
+      };
+      auto request = [&](const CUtensorMap& map, uint8_t* dst, uint64_t* bar, int y) {
+        if (lane == 0) mbar_arrive_expect_tx(bar, S::kTileKV);
         __syncwarp();
-        if (lane < boxes) tma_load_2d(ring + st * S::kTileKV + lane * box * 128, &map, &full[st], 0, y);
-        ++count;
+        if (lane < boxes) tma_load_2d(dst + lane * box * 128, &map, bar, 0, y);
+      };
+      auto request_k = [&](int y) {
+        const int st = k_count % kStages;
+        if (!wait(&k_empty[c * kStages + st], ((uint32_t)(k_count / kStages) & 1) ^ 1)) return;
+        request(map_k, k_ring + st * S::kTileKV, &k_full[c * kStages + st], y);
+        ++k_count;
+      };
+      int raws = 0;
+      // the values of step j, whose item sees keys [lo, hi)
+      auto request_v = [&](int y, int j, int lo, int hi) {
+        const int st = v_count % kStages, key0 = j * kCacheStep;
+        uint64_t* full = &v_full[c * kStages + st];
+        uint8_t* dst = v_ring + st * S::kTileKV;
+        if (!wait(&v_empty[c * kStages + st], ((uint32_t)(v_count / kStages) & 1) ^ 1)) return;
+        if (key0 >= lo && key0 + kCacheStep <= hi) {
+          request(map_v, dst, full, y);
+        } else {
+          // rows that no row of the item may see: zero (the other stages cover the time this takes)
+          request(map_v, dst, &raw[c], y);
+          if (!wait(&raw[c], (uint32_t)raws++ & 1)) return;
+          // 16-byte chunks; the swizzle stays within a row
+          for (int k = lane; k < (lo - key0) * 8; k += 32) *reinterpret_cast<uint4*>(dst + k * 16) = make_uint4(0, 0, 0, 0);
+          for (int k = max(hi - key0, 0) * 8 + lane; k < kCacheStep * 8; k += 32)
+            *reinterpret_cast<uint4*>(dst + k * 16) = make_uint4(0, 0, 0, 0);
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        }
+        ++v_count;
       };
       int v_y = -1;  // pool row (lane b: of box b) of the step whose values are requested next
       for (;; ++r) {
-        CacheRun run;
-        run.head = -1;
-        if (w.valid) {
-          run.tok = w.it.s.tok + w.it.tok0;
-          run.ntok = w.it.ntok;
-          run.pos0 = w.it.s.total - w.it.s.n + w.it.tok0;
-          run.total = w.it.s.total;
-          run.a0 = w.a0;
-          run.a1 = w.a1;
-          run.head = w.it.head;
-          run.slot = w.whole() ? -1 : 2 * worker + w.slot();
-          run.lo = w.it.lo;
-          run.hi = w.it.hi;
-        }
         const int qb = c * kBufs + r % kBufs;
-        if (r >= kBufs)
-          ok = ok && mbar_wait_warp(&q_empty[qb], (uint32_t)(r / kBufs - 1) & 1, args.status, kErrWaitProducer, abort_flag);
-        if (!ok) break;
+        if (r >= kBufs && !wait(&q_empty[qb], (uint32_t)(r / kBufs - 1) & 1)) break;
         if (lane == 0) {
+          CacheRun run;
+          run.head = -1;
+          if (w.valid) {
+            run.tok = w.it.s.tok + w.it.tok0;
+            run.ntok = w.it.ntok;
+            run.pos0 = w.it.s.total - w.it.s.n + w.it.tok0;
+            run.total = w.it.s.total;
+            run.a0 = w.a0;
+            run.a1 = w.a1;
+            run.head = w.it.head;
+            run.slot = w.whole() ? -1 : 2 * worker + w.slot();
+            run.lo = w.it.lo;
+            run.hi = w.it.hi;
+            run.seq = w.it.r;
+            if (run.slot >= 0 && w.slot() == 1)
+              *cache_record(args, worker) = {w.parts(), run.tok, run.ntok, run.head};
+          }
           runs[r % kCtRuns] = run;
           if (run.head < 0) {
             mbar_arrive(&q_full[qb]);
           } else {
-            if (run.slot >= 0 && w.slot() == 1)
-              *cache_record(args, worker) = {w.parts(), run.tok, run.ntok, run.head};
             const int tiles = SHARED ? (run.ntok + tile_frames - 1) / tile_frames : 1;
             mbar_arrive_expect_tx(&q_full[qb], tiles * tile_frames * args.group * 128);
             for (int x = 0; x < tiles; ++x)
@@ -301,15 +338,16 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           }
         }
         __syncwarp();
-        if (run.head < 0) break;
-        const int32_t* table = args.table + (int64_t)w.it.r * args.table_stride;
-        const int hi = run.hi, lo = run.lo, head = run.head, a1 = run.a1;
+        const CacheRun& run = runs[r % kCtRuns];
+        const int hi = run.hi, lo = run.lo, head = run.head, a0 = run.a0, a1 = run.a1;
+        if (head < 0) break;
+        const int32_t* table = args.table + (int64_t)run.seq * args.table_stride;
         auto look_up = [&](int j) {  // lane b: page of box b; -1: no row sees a key of it
           const int key = j * kCacheStep + lane * box;
           return lane < boxes && j < a1 && key < hi && key + box > lo ? table[key >> args.page_log2] : -1;
         };
-        int p = look_up(run.a0);
-        for (int j = run.a0; j < a1 && ok; ++j) {
+        int p = look_up(a0);
+        for (int j = a0; j < a1 && ok; ++j) {
           const int next = look_up(j + 1);  // a step ahead of its use
           const int key = j * kCacheStep + lane * box;
           int y = nowhere;
@@ -318,15 +356,17 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           else if (lane < boxes && key < hi && key + box > lo)
             record_error(args.status, kErrBadArgs);
           p = next;
-          request(map_k, k_ring, k_full + c * kStages, k_empty + c * kStages, k_count, y);
-          // values a step behind the keys: their stage falls free later
-          if (v_count < k_count - 1)
-            request(map_v, v_ring, v_full + c * kStages, v_empty + c * kStages, v_count, v_y);
+          request_k(y);
+          if (j > a0) request_v(v_y, j - 1, lo, hi);  // a step behind the keys: their stage falls free later
           v_y = y;
         }
         // the run's last values before its successor's Q, which waits for this run's last S
-        if (ok) request(map_v, v_ring, v_full + c * kStages, v_empty + c * kStages, v_count, v_y);
-        w.advance(args, tpt);
+        request_v(v_y, a1 - 1, lo, hi);
+        if (!ok) {
+          ++r;
+          break;
+        }
+        if (lane == 0) w.advance(args, tpt);
       }
       if (!ok && lane == 0) {
         // a wait gave up: let the copies in flight land before shared memory is given back
@@ -338,6 +378,9 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         };
         land(k_full + c * kStages, k_count);
         land(v_full + c * kStages, v_count);
+        if (raws)
+          while (!mbar_try_wait(&raw[c], (uint32_t)(raws - 1) & 1) && global_ns() - t0 < kWaitLimitNs) {
+          }
         for (int k = max(0, r - kBufs); k < r; ++k)
           while (!mbar_try_wait(&q_full[c * kBufs + k % kBufs], (uint32_t)(k / kBufs) & 1) &&
                  global_ns() - t0 < kWaitLimitNs) {
@@ -359,7 +402,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
     const int frame = row / args.group, sub = row - frame * args.group;  // frame of the tile, query head of the group
     const int i = (SHARED ? x * tile_frames : 0) + frame;                // frame of the item
     uint32_t g = 0;                                                      // the tile's steps so far
-    int vbase = 0;                                                       // the channel's steps before the run
     // the last run's row, whose epilogue is deferred: where it goes (nothing if null) and whether it is a part
     void* dst = nullptr;
     bool dst_part = false, pending = false;
@@ -418,7 +460,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             for (int k = 0; k < 8; ++k) reinterpret_cast<uint4*>(to)[k] = make_uint4(0, 0, 0, 0);
           }
         }
-        vbase += run.a1 - run.a0;
         continue;
       }
       const bool warp_live = __any_sync(0xffffffffu, live);
@@ -427,20 +468,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       const int hi = !live ? INT_MAX : args.causal ? min(max(run.pos0 + i + 1, 0), run.total) : run.total;
       const int lo = live && args.window ? max(run.pos0 + i + 1 - args.window, 0) : 0;
       float m_run = -INFINITY, l_run = 0.f;
-      // this warp's quarter of the V rows of step j that no row of the item may see
-      auto zero_values = [&](int j) {
-        const int count = vbase + j - run.a0, st = count % kStages, key0 = j * kCacheStep;
-        if (!mbar_wait_warp(&v_full[c * kStages + st], (uint32_t)(count / kStages) & 1, args.status, kErrWaitSoftmax,
-                            abort_flag))
-          return false;
-        uint8_t* vb = smem + S::kKV + (c * 2 * kStages + kStages + st) * S::kTileKV;
-        for (int k = row; k < kCacheStep * 8; k += 128) {  // 16-byte chunks; the swizzle stays within a row
-          const int key = key0 + (k >> 3);
-          if (key < run.lo || key >= run.hi) *reinterpret_cast<uint4*>(vb + k * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_async_smem();
-        return true;
-      };
       for (int j = b; j < e; ++j, ++g) {
         if (!(ok = mbar_wait_warp(&s_full[x], g & 1u, args.status, kErrWaitSoftmax, abort_flag))) break;
         tc_fence_after();
@@ -455,7 +482,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             break;
           tc_fence_after();
           if (j == b && pending) finish();
-          if ((j * 64 < run.lo || j * 64 + 64 > run.hi) && !(ok = zero_values(j))) break;
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&p_full[x]);
@@ -466,8 +492,8 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_free[x]);
-        const int kmax = hi - j * 64, kmin = lo - j * 64;
-        if (kmax < 64 || kmin > 0) {
+        if (__any_sync(0xffffffffu, j * 64 + 64 > hi || j * 64 < lo)) {  // some row does not see all keys
+          const int kmax = hi - j * 64, kmin = lo - j * 64;
 #pragma unroll
           for (int k = 0; k < 64; ++k)
             if (k >= kmax || k < kmin) sc[k] = -INFINITY;
@@ -536,7 +562,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           tmem_st16(tP + 16, packed);
         }
         l_run = l_run * alpha + (l2.x + l2.y);
-        if ((j * 64 < run.lo || j * 64 + 64 > run.hi) && !(ok = zero_values(j))) break;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -559,7 +584,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         }
       }
       pending = true;
-      vbase += run.a1 - run.a0;
     }
     if (ok && pending && mbar_wait_warp(&p_free[x], (g - 1) & 1u, args.status, kErrWaitSoftmax, abort_flag)) {
       tc_fence_after();

@@ -49,6 +49,7 @@ struct CacheAttnArgs {
   int causal, window;   // window 0: unlimited
   int split;            // 1: shares may end inside an item
   int min_share;        // least steps of a share
+  int whole_from;       // items stay whole where a share holds this many of the longest
   int rows_above, rows_upto;  // this launch's sequences: rows_above < new frames x group <= rows_upto
   float scale_log2;     // softmax scale x log2(e)
 };
@@ -136,7 +137,7 @@ __device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t l
 
 // The line's scan, by all `threads` threads of the CTA: prefix[r] = steps before sequence r, prefix[n_seqs] =
 // the line's length. Returns whether shares end inside items: not where the host rules it out, nor where a share
-// holds at least 16 of the longest items (whole items are then at most 1/16 uneven, and there is nothing to join).
+// holds whole_from of the longest items (whole items are then at most 1 / whole_from uneven, nothing is joined).
 // `part` holds 32 int64 of scratch. Ends with a CTA barrier.
 __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int threads, int ctas, int64_t* prefix,
                                            int64_t* part) {
@@ -172,7 +173,7 @@ __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int 
   }
   for (int r = r0; r < r1; ++r) prefix[r] += before;
   if (threadIdx.x == 0) prefix[a.n_seqs] = length;
-  return __syncthreads_or(a.split && longest * (int64_t)16 > cache_share(a, length, ctas));
+  return __syncthreads_or(a.split && longest * (int64_t)a.whole_from > cache_share(a, length, ctas));
 }
 
 // The runs of steps that one CTA works on, in order.
