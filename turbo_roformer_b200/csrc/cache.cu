@@ -433,24 +433,27 @@ int launch_cache_attention(const Layout& l, int page, const void* k, const void*
     return rc ? rc : make_tensor_map(&mv, prec, v, 2, dims, strides, box);
   };
   CUtensorMap mk, mv;
-  int rc = maps(kCrKeys, mk, mv);
-  if (rc) return rc;
+  int rc;
   float* const ws2 = a.ws ? a.ws + l.floats : nullptr;
-  a.whole_from = 16;
-  a.rows_above = 0;
-  a.rows_upto = l.tiles ? kFewRows : INT_MAX;
-  rc = l.rows == 16 ? launch_rows<T, 1>(mk, mv, a, l.workers, st) : launch_rows<T, 2>(mk, mv, a, l.workers, st);
-  if (rc) return rc;
   if (l.tiles) {
     CacheAttnArgs b = a;
     b.rows_above = kFewRows;
     b.rows_upto = INT_MAX;
+    b.run_cost = 2;
     b.whole_from = 6;  // a divided tile leaves 34 KB or more in the workspace
     b.ws = ws2;
     if ((rc = maps(kCacheStep, mk, mv))) return rc;
     rc = l.shared ? launch_tiles<T, true>(mk, mv, b, sms, st) : launch_tiles<T, false>(mk, mv, b, sms, st);
     if (rc) return rc;
   }
+  a.run_cost = 1;
+  a.whole_from = 16;
+  a.rows_above = 0;
+  a.rows_upto = l.tiles ? kFewRows : INT_MAX;
+  a.second = l.tiles;
+  if ((rc = maps(kCrKeys, mk, mv))) return rc;
+  rc = l.rows == 16 ? launch_rows<T, 1>(mk, mv, a, l.workers, st) : launch_rows<T, 2>(mk, mv, a, l.workers, st);
+  if (rc) return rc;
   if (!a.split) return TRC_OK;
   const CacheJoin j = {l.workers, l.rows, l.rows2, ws2};
   return launch("cache attention join", cache_join_kernel<T>, dim3(l.workers + kJoinBlocks * l.workers2), 256, 0, st,
@@ -626,6 +629,7 @@ int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const 
   a.n_pages = n_pages;
   a.causal = causal != 0;
   a.window = window > 1 << 30 ? 0 : window;  // longer than any sequence
+  a.second = 0;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.split = max_total > TRC_CACHE_MAX_WHOLE;
   a.min_share = a.split ? 2 : 1;  // steps: a part of less than 128 keys costs more to join than it saves

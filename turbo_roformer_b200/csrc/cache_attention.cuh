@@ -94,11 +94,12 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
-  grid_wait();
+  // Behind a cache_tiles_kernel this launch need not wait to begin: that one's blocks have all waited for what came
+  // before them, and it takes other rows and another workspace. It fills the SMs that the other leaves, and waits for
+  // it at its own end, so that whatever follows has both behind it.
+  cache_prefetch(args);
+  if (!args.second) grid_wait();
   grid_release();
-  // the first table lines travel while the lengths are read
-  if ((int64_t)threadIdx.x * 32 < (int64_t)args.n_seqs * args.table_stride)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(args.table + threadIdx.x * 32));
   const int tpt = kRows / args.group;
   // its barriers cover the initialisation above
   const int workers = gridDim.x * kCrWarps, worker = warp * gridDim.x + blockIdx.x;
@@ -107,7 +108,10 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
   CacheWalk cons;
   cons.begin(args, tpt, prefix, worker, workers, split);
   if (args.split && lane == 0) cache_record(args, worker)->parts = 0;
-  if (!cons.valid) return;
+  if (!cons.valid) {
+    if (args.second) grid_wait();
+    return;
+  }
   bool ok = true;
 
   // ---- loads. The warp's next tile: pj of a run that ends before tile p_end and sees keys [p_lo, p_hi); lane b holds
@@ -352,7 +356,7 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
     const bool whole = cons.whole();
     float* slot = whole ? nullptr : cache_slot(args, kRows, workers, 2 * worker + cons.slot());
     if (!whole && cons.slot() == 1 && lane == 0)
-      *cache_record(args, worker) = {cons.parts(), it.s.tok + it.tok0, it.ntok, it.head};
+      *cache_record(args, worker) = {cons.parts(args), it.s.tok + it.tok0, it.ntok, it.head};
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -383,12 +387,14 @@ __global__ void __launch_bounds__(32 * kCrWarps, 2)
       while (!mbar_try_wait(&full[k % kCrStages], (uint32_t)(k / kCrStages) & 1) && global_ns() - t0 < kWaitLimitNs) {
       }
   }
+  if (args.second) grid_wait();
 }
 
-// Joins the parts of items that were divided among workers, for one launch's workers (0 .. workers - 1) and, behind
-// them, a second launch's with a workspace of its own. A block takes the item that its worker began and did not end, if
-// there is one (kJoinBlocks of them share the rows of one of the second launch's). A warp takes a row at a time and reads two parts at once (16 lanes x 4 dims each); where an item
-// has few rows in many parts, 2, 4 or 8 warps share a row and meet in shared memory.
+// Joins the parts of items that were divided among workers, for the workers of cache_rows_kernel (0 .. workers - 1) and,
+// behind them, those of cache_tiles_kernel, with a workspace of its own. A block takes the item that its worker began
+// and did not end, if there is one. Few rows: a warp takes a row at a time and reads two parts at once (16 lanes x 4
+// dims each); where an item has few rows in many parts, 2, 4 or 8 warps share a row and meet in shared memory. Tiles:
+// kJoinBlocks blocks share an item, a thread takes 4 dims of a row, consecutive threads consecutive rows.
 constexpr int kJoinBlocks = 8;
 struct CacheJoin {
   int workers, rows;  // of the first launch; rows of its slots
@@ -406,6 +412,19 @@ struct JoinSum {
     o = make_float4(o.x * f1 + x.x * f2, o.y * f1 + x.y * f2, o.z * f1 + x.z * f2, o.w * f1 + x.w * f2);
   }
 };
+// dims d .. d + 3 of a joined row
+template <typename T>
+__device__ __forceinline__ void join_store(const CacheAttnArgs& args, const CacheRecord& rec, int row, int d,
+                                           const JoinSum& s) {
+  const int i = row / args.group, head = rec.head * args.group + (row - i * args.group);
+  const int64_t tok = rec.tok + i;
+  const float gate = args.gates ? args.gates[tok * args.hq + head] : 1.f;
+  const float f = s.l == 0.f ? 0.f : gate / s.l;  // no visible key: zero
+  uint2 u;
+  u.x = OperandType<T>::pack2(s.o.x * f, s.o.y * f);
+  u.y = OperandType<T>::pack2(s.o.z * f, s.o.w * f);
+  *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + tok * args.out_stride + head * 64 + d) = u;
+}
 template <typename T>
 __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__ CacheAttnArgs first,
                                                          const __grid_constant__ CacheJoin j) {
@@ -426,6 +445,22 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
   const CacheRecord rec = *cache_record(args, worker);
   if (rec.parts == 0) return;
   const int rows = rec.ntok * args.group;
+  if (ny > 1) {
+    const int padded = (rows + 31) & ~31;
+    for (int x = y * 256 + threadIdx.x; x < 16 * padded; x += ny * 256) {
+      const int k = x / padded, row = x - k * padded;
+      if (row >= rows) continue;
+      JoinSum s = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 4
+      for (int p = 0; p < rec.parts; ++p) {
+        const float* src = cache_slot(args, tile_rows, workers, 2 * (worker + p) + (p == 0 ? 1 : 0));
+        const float2 ml = *reinterpret_cast<const float2*>(src + tile_rows * 64 + row * 2);
+        s.add(ml.x, ml.y, *reinterpret_cast<const float4*>(src + (k * tile_rows + row) * 4));
+      }
+      join_store<T>(args, rec, row, k * 4, s);
+    }
+    return;
+  }
   const int share = rec.parts <= 4 || rows > 4 ? 1 : rows > 2 ? 2 : rows > 1 ? 4 : 8;  // warps per row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane >> 4, d = (lane & 15) * 4;
@@ -458,16 +493,7 @@ __global__ void __launch_bounds__(256) cache_join_kernel(const __grid_constant__
         for (int w = warp + 1; w < warp + share; ++w) s.add(meet_ml[w][lane].x, meet_ml[w][lane].y, meet_o[w][lane]);
       __syncthreads();
     }
-    if (row < rows && warp % share == 0 && sub == 0) {
-      const int i = row / args.group, head = rec.head * args.group + (row - i * args.group);
-      const int64_t tok = rec.tok + i;
-      const float gate = args.gates ? args.gates[tok * args.hq + head] : 1.f;
-      const float f = s.l == 0.f ? 0.f : gate / s.l;
-      uint2 u;
-      u.x = OperandType<T>::pack2(s.o.x * f, s.o.y * f);
-      u.y = OperandType<T>::pack2(s.o.z * f, s.o.w * f);
-      *reinterpret_cast<uint2*>(static_cast<T*>(args.out) + tok * args.out_stride + head * 64 + d) = u;
-    }
+    if (row < rows && warp % share == 0 && sub == 0) join_store<T>(args, rec, row, d, s);
   }
 }
 

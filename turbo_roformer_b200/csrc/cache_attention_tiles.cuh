@@ -52,7 +52,8 @@ struct CtSmem {
   static constexpr int kQ = 0;                                                          // [bufs][tiles]
   static constexpr int kKV = kQ + kQBufs * kCtTiles * kTileQ;                                    // [channels][K, V][stages]
   static constexpr int kScale = kKV + kChannels * 2 * kStages * kTileKV;                // [tiles][128] fp32
-  static constexpr int kRun = kScale + kCtTiles * 128 * 4;                              // [channels][kCtRuns]
+  static constexpr int kOut = kScale + kCtTiles * 128 * 4;                              // [softmax warps][8 rows]
+  static constexpr int kRun = kOut + 4 * kCtTiles * 1024;                               // [channels][kCtRuns]
   static constexpr int kWalk = kRun + kChannels * kCtRuns * (int)sizeof(CacheRun);      // [channels] CacheWalk
   static constexpr int kBar = kWalk + kChannels * 128;
   static constexpr int kScan = kBar + 768 + 256;
@@ -70,6 +71,62 @@ struct CtSmem {
   static_assert(kBar % 8 == 0 && kScan % 8 == 0, "alignment");
   static_assert(kScan + (kCacheMaxSeqs + 1) * 8 + 1024 <= 232448, "shared memory per CTA");
 };
+
+// A warp's rows of O from TMEM to where they go (thread = row, dst null: nowhere), and the accumulator's release. A
+// function of its own, because inlined into the softmax loop its registers cost every step (1.36 instead of 1.15 us).
+template <typename TIn, int ROWS>
+__device__ __noinline__ void ct_finish(uint32_t t_o, void* dst, bool is_part, float scale, uint8_t* stage,
+                                       uint64_t* o_free) {
+  const int lane = threadIdx.x & 31;
+  if (is_part) {
+    // a part: 4 dims of 32 consecutive rows per store
+#pragma unroll 1
+    for (int hc = 0; hc < 2; ++hc) {
+      float o[32];
+      tmem_ld32(t_o + hc * 32, o);
+      float4* d = static_cast<float4*>(dst) + hc * 8 * ROWS;
+      if (dst) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) d[k * ROWS] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      }
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(o_free);
+    return;
+  }
+  // results: eight rows at a time through shared memory, so that a store instruction writes whole 128-byte rows (a
+  // thread's own row in 16-byte pieces would touch 32 lines per instruction)
+  uint32_t u[32];
+#pragma unroll
+  for (int hc = 0; hc < 2; ++hc) {
+    float o[32];
+    tmem_ld32(t_o + hc * 32, o);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) u[hc * 16 + k] = OperandType<TIn>::pack2(o[2 * k] * scale, o[2 * k + 1] * scale);
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(o_free);
+#pragma unroll 1
+  for (int q = 0; q < 4; ++q) {
+    if ((lane >> 3) == q) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        *reinterpret_cast<uint4*>(stage + (lane & 7) * 128 + ((k ^ (lane & 7)) << 4)) =
+            make_uint4(u[4 * k], u[4 * k + 1], u[4 * k + 2], u[4 * k + 3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r8 = h * 4 + (lane >> 3), k = lane & 7;
+      uint4* to = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), q * 8 + r8));
+      const uint4 v = *reinterpret_cast<const uint4*>(stage + r8 * 128 + ((k ^ r8) << 4));
+      if (to) to[k] = v;
+    }
+    __syncwarp();
+  }
+}
 
 template <typename TIn, bool SHARED>
 __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
@@ -129,12 +186,12 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
   }
+  cache_prefetch(args);
   if (warp == 3) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  // No wait here: this launch follows a cache_rows_kernel whose blocks have all waited for what came before them, and
-  // takes other rows and another workspace than it. It waits for that launch at its own end.
+  grid_wait();
   grid_release();
   const bool split = cache_scan(args, tpt, S::kThreads, workers, prefix, part);
   tc_fence_before();
@@ -261,7 +318,9 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       CacheWalk& w = *reinterpret_cast<CacheWalk*>(smem + S::kWalk + c * 128);
       static_assert(sizeof(CacheWalk) <= 128, "layout");
       if (lane == 0) {
-        w.begin(args, tpt, prefix, worker, workers, split);
+        CacheWalk first;
+        first.begin(args, tpt, prefix, worker, workers, split);
+        w = first;
         if (args.split) cache_record(args, worker)->parts = 0;
       }
       bool ok = true;
@@ -324,7 +383,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             run.hi = w.it.hi;
             run.seq = w.it.r;
             if (run.slot >= 0 && w.slot() == 1)
-              *cache_record(args, worker) = {w.parts(), run.tok, run.ntok, run.head};
+              *cache_record(args, worker) = {w.parts(args), run.tok, run.ntok, run.head};
           }
           runs[r % kCtRuns] = run;
           if (run.head < 0) {
@@ -366,7 +425,11 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           ++r;
           break;
         }
-        if (lane == 0) w.advance(args, tpt);
+        if (lane == 0) {
+          CacheWalk next = w;
+          next.advance(args, tpt);
+          w = next;
+        }
       }
       if (!ok && lane == 0) {
         // a wait gave up: let the copies in flight land before shared memory is given back
@@ -402,32 +465,12 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
     const int frame = row / args.group, sub = row - frame * args.group;  // frame of the tile, query head of the group
     const int i = (SHARED ? x * tile_frames : 0) + frame;                // frame of the item
     uint32_t g = 0;                                                      // the tile's steps so far
-    // the last run's row, whose epilogue is deferred: where it goes (nothing if null) and whether it is a part
+    // the last run's row, whose epilogue is deferred: where it goes (nowhere if null), and whether it is a part
     void* dst = nullptr;
     bool dst_part = false, pending = false;
+    uint8_t* out_stage = smem + S::kOut + (warp - S::kSoftmax0) * 1024;
     auto finish = [&]() {
-      const float scale = dst_part ? 1.f : *row_scale;
-#pragma unroll 1
-      for (int hc = 0; hc < 2; ++hc) {
-        float o[32];
-        tmem_ld32(tO + hc * 32, o);
-        if (hc == 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&o_free[x]);
-        }
-        if (dst) {
-          if (dst_part) {
-            float4* d = static_cast<float4*>(dst) + hc * 8;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) d[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] *= scale;
-            store32<TIn>(static_cast<TIn*>(dst) + hc * 32, o);
-          }
-        }
-      }
+      ct_finish<TIn, S::kRows>(tO, dst, dst_part, *row_scale, out_stage, &o_free[x]);
       pending = false;
     };
     bool ok = true;
@@ -453,7 +496,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             *reinterpret_cast<float2*>(slot + S::kRows * 64 + slot_row * 2) = make_float2(-INFINITY, 0.f);
 #pragma unroll 1
             for (int k = 0; k < 16; ++k)
-              reinterpret_cast<float4*>(slot + slot_row * 64)[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+              reinterpret_cast<float4*>(slot)[k * S::kRows + slot_row] = make_float4(0.f, 0.f, 0.f, 0.f);
           } else {
             TIn* to = static_cast<TIn*>(args.out) + tok * args.out_stride + head * 64;
 #pragma unroll 1
@@ -578,7 +621,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         if (dst_part) {
           float* slot = cache_slot(args, S::kRows, workers, run.slot);
           *reinterpret_cast<float2*>(slot + S::kRows * 64 + slot_row * 2) = make_float2(m_run, l_run);
-          dst = slot + slot_row * 64;
+          dst = slot + slot_row * 4;
         } else {
           dst = static_cast<TIn*>(args.out) + tok * args.out_stride + head * 64;
         }
@@ -597,7 +640,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
-  grid_wait();
 }
 
 }  // namespace trc

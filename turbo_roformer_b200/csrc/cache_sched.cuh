@@ -4,11 +4,13 @@
 // The work is a list of items, one per (sequence, row tile, cache head): a row tile is up to `tpt` new frames
 // with all `group` query heads that share the cache head. An item is a run of 64-key steps that covers the
 // keys some row of it may see. Steps of all items form one line in the order (sequence, row tile, head,
-// step); every CTA takes an equal share of it, whatever the lengths are, so ragged batches, few heads over
-// long caches and many heads over short ones all fill the GPU alike. Where a share ends inside an item the
-// item's parts go to the workspace as (unnormalised sum, maximum, weight) per row and a second kernel joins
-// them in the order of the keys, so results do not depend on timing. A CTA owns two workspace slots: one for
-// a first item begun by another CTA, one for a last item that it begins and does not end.
+// step); every worker (a CTA, a tile of one or a warp) takes an equal share of it, whatever the lengths are, so ragged
+// batches, few heads over long caches and many heads over short ones all fill the GPU alike. Where a share ends inside
+// an item the item's parts go to the workspace as (unnormalised sum, maximum, weight) per row and a second kernel joins
+// them in the order of the keys, so results do not depend on timing. A worker owns two workspace slots: one for a first
+// item begun by another, one for a last item that it begins and does not end.
+// An item also costs its set-up and its epilogue, whatever its length: on the line its steps are preceded by run_cost
+// places that stand for no step, so that shares of many short items come out as even as shares of few long ones.
 // Each CTA derives the line from the device's lengths (a scan over the sequences); the host needs only bounds.
 #pragma once
 
@@ -49,10 +51,20 @@ struct CacheAttnArgs {
   int causal, window;   // window 0: unlimited
   int split;            // 1: shares may end inside an item
   int min_share;        // least steps of a share
+  int run_cost;         // places of an item on the line besides its steps
   int whole_from;       // items stay whole where a share holds this many of the longest
   int rows_above, rows_upto;  // this launch's sequences: rows_above < new frames x group <= rows_upto
+  int second;           // 1: launched behind a kernel of the same call that takes the other sequences
   float scale_log2;     // softmax scale x log2(e)
 };
+
+// The lengths and the first table lines into L2, before grid_wait: L2 is where earlier kernels' writes to them arrive.
+__device__ __forceinline__ void cache_prefetch(const CacheAttnArgs& a) {
+  const int64_t x = (int64_t)threadIdx.x * 32;
+  if (x <= a.n_seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.cu + x));
+  if (x < a.n_seqs) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.total + x));
+  if (x < (int64_t)a.n_seqs * a.table_stride) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.table + x));
+}
 
 struct CacheSeq {
   int tok, n, total;  // first row, new frames, frames in the cache
@@ -84,8 +96,9 @@ struct CacheItem {
   int tok0, ntok;     // its new frames (within the sequence)
   int lo, hi;         // keys that some row sees
   int t0, t1;         // its steps
-  int64_t start;      // place of its first step on the line
+  int64_t start;      // its place on the line
 
+  __device__ __forceinline__ int places(const CacheAttnArgs& a) const { return t1 - t0 + a.run_cost; }
   __device__ __forceinline__ void set_tile(const CacheAttnArgs& a, int tpt) {
     tok0 = tile * tpt;
     ntok = min(tpt, s.n - tok0);
@@ -106,15 +119,15 @@ struct CacheItem {
     int64_t left = at - prefix[r];
     for (tile = 0;; ++tile) {
       set_tile(a, tpt);
-      const int64_t all = (int64_t)(t1 - t0) * a.hkv;
+      const int64_t all = (int64_t)places(a) * a.hkv;
       if (left < all) break;
       left -= all;
     }
-    head = (int)div_pos(left, t1 - t0);
-    start = at - (left - (int64_t)head * (t1 - t0));
+    head = (int)div_pos(left, places(a));
+    start = at - (left - (int64_t)head * places(a));
   }
   __device__ __forceinline__ void next(const CacheAttnArgs& a, int tpt) {
-    start += t1 - t0;
+    start += places(a);
     if (++head < a.hkv) return;
     head = 0;
     if (tok0 + ntok < s.n) {
@@ -135,7 +148,7 @@ __device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t l
   return max(div_pos(length + ctas - 1, ctas), (int64_t)a.min_share);
 }
 
-// The line's scan, by all `threads` threads of the CTA: prefix[r] = steps before sequence r, prefix[n_seqs] =
+// The line's scan, by all `threads` threads of the CTA: prefix[r] = places before sequence r, prefix[n_seqs] =
 // the line's length. Returns whether shares end inside items: not where the host rules it out, nor where a share
 // holds whole_from of the longest items (whole items are then at most 1 / whole_from uneven, nothing is joined).
 // `part` holds 32 int64 of scratch. Ends with a CTA barrier.
@@ -151,8 +164,8 @@ __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int 
     int64_t steps = 0;
     for (it.tile = 0; it.tile * tpt < it.s.n; ++it.tile) {
       it.set_tile(a, tpt);
-      steps += it.t1 - it.t0;
-      longest = max(longest, it.t1 - it.t0);
+      steps += it.places(a);
+      longest = max(longest, it.places(a));
     }
     prefix[r] = sum;
     sum += steps * a.hkv;
@@ -176,52 +189,57 @@ __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int 
   return __syncthreads_or(a.split && longest * (int64_t)a.whole_from > cache_share(a, length, ctas));
 }
 
-// The runs of steps that one CTA works on, in order.
+// The runs of steps that one worker works on, in order.
 struct CacheWalk {
   CacheItem it;
-  int64_t s0, s1;  // the CTA's share of the line
+  int64_t s0, s1;  // the worker's share of the line
   int a0, a1;      // the run's steps [a0, a1) within the item
   bool split, valid;
 
-  __device__ __forceinline__ void set_run() {
-    a0 = it.t0;
-    a1 = it.t1;
-    if (split) {
-      if (it.start < s0) a0 += (int)(s0 - it.start);
-      if (it.start + (it.t1 - it.t0) > s1) a1 = it.t0 + (int)(s1 - it.start);
-    }
-  }
-  __device__ __forceinline__ void begin(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int cta, int ctas,
+  __device__ __forceinline__ void begin(const CacheAttnArgs& a, int tpt, const int64_t* prefix, int worker, int workers,
                                         bool divided) {
-    const int64_t length = prefix[a.n_seqs], w = cache_share(a, length, ctas);
+    const int64_t length = prefix[a.n_seqs], w = cache_share(a, length, workers);
     split = divided;
-    s0 = min(length, (int64_t)cta * w);
+    s0 = min(length, (int64_t)worker * w);
     s1 = min(length, s0 + w);
     valid = s0 < s1;
     if (!valid) return;
     it.seek(a, tpt, prefix, s0);
-    if (!split && it.start < s0) it.next(a, tpt);  // whole items go to the CTA whose share holds their start
-    valid = it.start < s1;
-    if (valid) set_run();
+    if (!split && it.start < s0) it.next(a, tpt);  // whole items go to the worker whose share holds their start
+    settle(a, tpt);
   }
   __device__ __forceinline__ void advance(const CacheAttnArgs& a, int tpt) {
     it.next(a, tpt);
-    valid = it.start < s1;
-    if (valid) set_run();
+    settle(a, tpt);
+  }
+  // the next item from `it` on of which a step lies in the share
+  __device__ __forceinline__ void settle(const CacheAttnArgs& a, int tpt) {
+    for (;; it.next(a, tpt)) {
+      valid = it.start < s1;
+      if (!valid) return;
+      a0 = it.t0;
+      a1 = it.t1;
+      if (!split) return;
+      const int64_t first = it.start + a.run_cost;  // place of step t0
+      a0 += (int)max(s0 - first, (int64_t)0);
+      a1 = (int)min((int64_t)a1, it.t0 + max(s1 - first, (int64_t)0));
+      if (a0 < a1) return;
+    }
   }
   __device__ __forceinline__ bool whole() const { return a0 == it.t0 && a1 == it.t1; }
   __device__ __forceinline__ int slot() const { return a0 == it.t0 ? 1 : 0; }  // of a run that is not whole
-  // CTAs that work on this item, when it is begun here and not ended
-  __device__ __forceinline__ int parts() const {
+  // workers on this item, when it is begun here and not ended
+  __device__ __forceinline__ int parts(const CacheAttnArgs& a) const {
     const int64_t w = s1 - s0;  // a share that an item outlasts is not the line's last, so it is a full one
-    return 1 + (int)div_pos(it.start + (it.t1 - it.t0) - 1 - s0, w);
+    return 1 + (int)div_pos(it.start + it.places(a) - 1 - s0, w);
   }
 };
 
-// Workspace: for each CTA a record of the item that it begins and does not end, then the slots. Slot
-// (2 cta + which) holds [rows][64] sums, then [rows][2] (maximum in log2 units, weight).
+// Workspace: for each worker a record of the item that it begins and does not end, then the slots. Slot
+// (2 worker + which) holds a run's sums, 64 per row, then [rows][2] (maximum in log2 units, weight). The sums are
+// [rows][64] where lanes hold columns (cache_rows_kernel) and [16][rows][4] where they hold rows (cache_tiles_kernel).
 struct CacheRecord {
-  int parts;  // CTAs that work on the item; 0: there is none
+  int parts;  // workers on the item; 0: there is none
   int tok, ntok, head;
 };
 __host__ __device__ __forceinline__ int64_t cache_slot_floats(int rows) { return (int64_t)rows * 66; }
