@@ -61,9 +61,10 @@ int page_log2_of(int page) {
 
 // ------------------------------------------------------------------------------------------------ plan
 // Every block repeats the scan over the sequences (two 64-bit sums per thread) and then takes its part of two
-// flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows. Nothing is
-// exchanged between blocks, so one launch serves any batch: a row's page is either fresh (read from the free
-// list, not from the table that another block is writing) or was in the table before.
+// flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows, four at a time (one
+// search, then onwards; vector stores). Nothing is exchanged between blocks, so one launch serves any batch: a row's
+// page is either fresh (read from the free list, not from the table that another block is writing) or was in the table
+// before. Lengths and sums sit in shared memory; the scan is a latency of some 3 us and bounds small batches.
 struct PlanArgs {
   const int32_t* cached;
   const int32_t* fresh;  // new lengths
@@ -91,30 +92,38 @@ __device__ __forceinline__ int last_upto(const int32_t* v, int n, int at) {
 
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_constant__ PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
-  int32_t* cu = plan_smem;                 // [n_seqs + 1] rows before each sequence
-  int32_t* base = plan_smem + a.n_seqs + 1;  // [n_seqs + 1] fresh pages before each sequence
+  int32_t* cu = plan_smem;                   // [n_seqs + 1] rows before each sequence
+  int32_t* base = cu + a.n_seqs + 1;         // [n_seqs + 1] fresh pages before each sequence
+  int32_t* cached = base + a.n_seqs + 1;     // [n_seqs] frames it has, 0 where the lengths are bad
   __shared__ int64_t part[2][kPlanThreads / 32];
   __shared__ int flags;
   if (threadIdx.x == 0) flags = 0;
   grid_wait();
   grid_release();
-  const int per = (a.n_seqs + kPlanThreads - 1) / kPlanThreads;
-  const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
-  int64_t rows = 0, pages = 0;
+  // the new lengths pass through cu
   int bad = 0;
-  auto lengths = [&](int r, int& c, int& n) {
-    c = a.cached[r];
-    n = a.fresh[r];
+  for (int r = threadIdx.x; r < a.n_seqs; r += kPlanThreads) {
+    int c = a.cached[r], n = a.fresh[r];
     if (c < 0 || n < 0 || (int64_t)c + n > (1 << 30)) {
       bad |= TRC_CACHE_BAD_LENGTH;
       c = n = 0;
     }
-  };
+    cached[r] = c;
+    cu[r] = n;
+    if (blockIdx.x == 0) {
+      a.total[r] = c + n;
+      if (pages_of((int64_t)c + n, a.page_log2) > a.table_stride) bad |= TRC_CACHE_TABLE_FULL;
+    }
+  }
+  __syncthreads();
+  // an odd number of sequences per thread: neighbours' strides then miss each other's banks
+  const int per = ((a.n_seqs + kPlanThreads - 1) / kPlanThreads) | 1;
+  const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
+  int64_t rows = 0, pages = 0;
+  auto pages_for = [&](int c, int n) { return pages_of((int64_t)c + n, a.page_log2) - pages_of(c, a.page_log2); };
   for (int r = r0; r < r1; ++r) {
-    int c, n;
-    lengths(r, c, n);
-    rows += n;
-    pages += pages_of((int64_t)c + n, a.page_log2) - pages_of(c, a.page_log2);
+    rows += cu[r];
+    pages += pages_for(cached[r], cu[r]);
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t rs = rows, ps = pages;
@@ -144,17 +153,11 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     all_pages += part[1][w];
   }
   for (int r = r0; r < r1; ++r) {
-    int c, n;
-    lengths(r, c, n);
+    const int n = cu[r];
     cu[r] = (int)min(rs, (int64_t)INT_MAX);
     base[r] = (int)min(ps, (int64_t)INT_MAX);
     rs += n;
-    ps += pages_of((int64_t)c + n, a.page_log2) - pages_of(c, a.page_log2);
-    if (blockIdx.x == 0) {
-      a.cu[r] = cu[r];
-      a.total[r] = c + n;
-      if (pages_of((int64_t)c + n, a.page_log2) > a.table_stride) bad |= TRC_CACHE_TABLE_FULL;
-    }
+    ps += pages_for(cached[r], n);
   }
   const int live_rows = (int)min(all_rows, (int64_t)INT_MAX), live_pages = (int)min(all_pages, (int64_t)INT_MAX);
   if (threadIdx.x == 0) {
@@ -167,31 +170,43 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     if (bad) atomicOr(&flags, bad);
   }
   __syncthreads();
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    a.cu[a.n_seqs] = live_rows;
-    a.counts[0] = min(live_pages, a.n_free);
-    a.counts[1] = flags;
+  if (blockIdx.x == 0) {
+    for (int r = threadIdx.x; r <= a.n_seqs; r += kPlanThreads) a.cu[r] = cu[r];
+    if (threadIdx.x == 0) {
+      a.counts[0] = min(live_pages, a.n_free);
+      a.counts[1] = flags;
+    }
   }
 
   const int stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + threadIdx.x;
   // fresh pages into the table
   for (int64_t e = first; e < live_pages; e += stride) {
     const int r = last_upto(base, a.n_seqs, (int)e);
-    int c, n;
-    lengths(r, c, n);
-    const int64_t column = (int64_t)pages_of(c, a.page_log2) + (e - base[r]);
+    const int64_t column = (int64_t)pages_of(cached[r], a.page_log2) + (e - base[r]);
     if (column < a.table_stride)
       a.table[(int64_t)r * a.table_stride + column] = e < a.n_free ? a.free_pages[e] : -1;
   }
-  // rows: position and slot
-  for (int64_t row = first; row < a.capacity; row += stride) {
-    int pos = 0, slot = -1;
-    if (row < live_rows) {
-      const int r = last_upto(cu, a.n_seqs, (int)row);
-      int c, n;
-      lengths(r, c, n);
-      pos = c + (int)(row - cu[r]);
-      const int column = pos >> a.page_log2, held = pages_of(c, a.page_log2);
+  // rows: position and slot, four to a thread
+  auto store4 = [&](int32_t* to, int64_t row0, const int(&v)[4]) {
+    if ((reinterpret_cast<uintptr_t>(to) & 15) == 0 && row0 + 4 <= a.capacity) {
+      *reinterpret_cast<int4*>(to + row0) = make_int4(v[0], v[1], v[2], v[3]);
+    } else {
+      for (int i = 0; i < 4 && row0 + i < a.capacity; ++i) to[row0 + i] = v[i];
+    }
+  };
+  for (int64_t row0 = 4ll * first; row0 < a.capacity; row0 += 4ll * stride) {
+    int pos[4], slot[4];
+    int r = row0 < live_rows ? last_upto(cu, a.n_seqs, (int)row0) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t row = row0 + i;
+      pos[i] = 0;
+      slot[i] = -1;
+      if (row >= live_rows) continue;
+      while (cu[r + 1] <= row) ++r;
+      const int c = cached[r];
+      pos[i] = c + (int)(row - cu[r]);
+      const int column = pos[i] >> a.page_log2, held = pages_of(c, a.page_log2);
       int page = -1;
       if (column < a.table_stride) {
         if (column < held) {
@@ -202,10 +217,10 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
         }
       }
       if (page >= 0 && page <= (INT_MAX >> a.page_log2))
-        slot = (page << a.page_log2) + (pos & ((1 << a.page_log2) - 1));
+        slot[i] = (page << a.page_log2) + (pos[i] & ((1 << a.page_log2) - 1));
     }
-    a.positions[row] = pos;
-    a.slots[row] = slot;
+    store4(a.positions, row0, pos);
+    store4(a.slots, row0, slot);
   }
 }
 
@@ -496,18 +511,18 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
   a.capacity = max_rows;
   const int sms = trc::sm_count();
   if (!sms) return set_last_error(TRC_E_CUDA, "cache plan: no current CUDA device");
-  const int smem = 2 * (n_seqs + 1) * 4;
+  const int smem = (3 * n_seqs + 2) * 4;
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!(done.load(std::memory_order_relaxed) >> (dev & 63) & 1)) {
     const cudaError_t e = cudaFuncSetAttribute(trc::cache_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               2 * (TRC_CACHE_PLAN_MAX_SEQS + 1) * 4);
+                                               (3 * TRC_CACHE_PLAN_MAX_SEQS + 2) * 4);
     if (e != cudaSuccess) return set_last_error(TRC_E_CUDA, cudaGetErrorString(e));
     done.fetch_or(1ull << (dev & 63));
   }
-  // blocks for the rows; the fresh pages are at most as many plus one per sequence
-  const int64_t most = (int64_t)max_rows + n_seqs;
+  // a thread for every four rows
+  const int64_t most = (int64_t)max_rows / 4 + 1;
   const int blocks = (int)((most + trc::kPlanThreads - 1) / trc::kPlanThreads);
   return trc::launch("cache plan", trc::cache_plan_kernel, dim3(blocks < 2 * sms ? blocks : 2 * sms), trc::kPlanThreads,
                      smem, (cudaStream_t)stream, a);

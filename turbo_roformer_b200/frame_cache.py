@@ -115,15 +115,17 @@ def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, fre
         raise ValueError(f"page must be one of {PAGES}")
     if not 0 <= max_rows <= _INT32_MAX:
         raise ValueError("max_rows out of range")
-    sizes = (n + 1, n, max_rows, max_rows, 2)
     if out is None:
-        out = CachePlan._make(cached.new_empty(2 * (n + max_rows) + 3).split_with_sizes(sizes))  # one allocation
+        # one allocation, the slots first: on a 16-byte boundary
+        slots, positions, cu, total, counts = cached.new_empty(2 * (max_rows + n) + 3).split_with_sizes(
+            (max_rows, max_rows, n + 1, n, 2))
+        out = CachePlan(cu, total, slots, positions, counts)
     else:
-        for t, size, name in zip(out, sizes, CachePlan._fields):
+        for t, size, name in zip(out, (n + 1, n, max_rows, max_rows, 2), CachePlan._fields):
             _ints(t, index, 1, name)
             if t.shape[0] != size:
                 raise ValueError(f"{name} must have {size} elements")
-    cu, total, slots, positions, counts = out
+        cu, total, slots, positions, counts = out
     _call(index, "trc_cache_plan", cached.data_ptr(), new.data_ptr(), n, page, free_pages.data_ptr(),
           free_pages.shape[0], table.data_ptr(), columns, max_rows, cu.data_ptr(), total.data_ptr(), slots.data_ptr(),
           positions.data_ptr(), counts.data_ptr())
