@@ -366,9 +366,8 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       int v_y = -1;  // pool row (lane b: of box b) of the step whose values are requested next
       for (;; ++r) {
         const int qb = c * kBufs + r % kBufs;
-        if (r >= kBufs && !wait(&q_empty[qb], (uint32_t)(r / kBufs - 1) & 1)) break;
+        CacheRun& run = runs[r % kCtRuns];
         if (lane == 0) {
-          CacheRun run;
           run.head = -1;
           if (w.valid) {
             run.tok = w.it.s.tok + w.it.tok0;
@@ -384,8 +383,13 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             run.seq = w.it.r;
             if (run.slot >= 0 && w.slot() == 1)
               *cache_record(args, worker) = {w.parts(args), run.tok, run.ntok, run.head};
+            // one buffer: Q is asked for only once its predecessor is done with; until then it comes as far as L2
+            if (kBufs == 1) tma_prefetch_3d(&map_q, 0, run.head * args.group, run.tok);
           }
-          runs[r % kCtRuns] = run;
+        }
+        __syncwarp();
+        if (r >= kBufs && !wait(&q_empty[qb], (uint32_t)(r / kBufs - 1) & 1)) break;
+        if (lane == 0) {
           if (run.head < 0) {
             mbar_arrive(&q_full[qb]);
           } else {
@@ -397,7 +401,6 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           }
         }
         __syncwarp();
-        const CacheRun& run = runs[r % kCtRuns];
         const int hi = run.hi, lo = run.lo, head = run.head, a0 = run.a0, a1 = run.a1;
         if (head < 0) break;
         const int32_t* table = args.table + (int64_t)run.seq * args.table_stride;
