@@ -439,6 +439,99 @@ def test_attention_on_another_stream_and_repeated(cuda_device, new):
         assert torch.equal(g, want)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new,total,heads,kv,page", [
+    ([200], [455], 12, 4, 16), ([60, 77, 3], [60, 700, 90], 10, 2, 128), ([26, 25, 51], [300, 26, 1000], 5, 1, 32),
+    ([7], [200], 64, 1, 64), ([3, 2, 9], [700, 20, 9], 99, 3, 16), ([129, 128, 127, 64, 33, 32], [700] * 6, 2, 2, 64)])
+def test_attention_tiles(cuda_device, dtype, new, total, heads, kv, page):
+    """Groups that do not divide a tile's 128 rows, tiles that end inside a sequence, batches that take both kernels."""
+    c = Case(dtype, new, total, heads, kv, page, pad=5, gates=True, seed=len(new))
+    c.check(causal=True)
+    c.check(causal=False, window=70)
+    c.check(causal=True, window=300)
+
+
+@pytest.mark.parametrize("new", [40, 150, 400])
+def test_attention_many_divided_items(cuda_device, new):
+    """Many cache heads, several items and parts of items to each worker of the tensor-core kernel, and the joins."""
+    c = Case("fp16", [new, new // 3], [900, 640], 200, 200, 64, gates=True)
+    c.check(causal=False)
+    c.check(causal=True)
+
+
+def test_attention_shared_pages(cuda_device):
+    """Two sequences whose tables name the same pages (a common beginning): both read them."""
+    c = Case("fp16", [1, 40], [300, 300], 2, 2, 32)
+    c.table[1, :6] = c.table[0, :6]
+    c.check()
+
+
+@pytest.mark.parametrize("new", [2, 60, 200])
+def test_pool_offsets_past_32_bits(cuda_device, new):
+    """Pages whose elements lie more than 2^31 (and bytes more than 2^32) into the pool, written and read."""
+    kv, page, n_pages, dt = 8, 128, 36000, torch.float16  # 2.4e9 elements per pool
+    k = torch.empty(n_pages, kv, page, 64, dtype=dt, device="cuda")
+    v = torch.empty_like(k)
+    c = Case("fp16", [new], [new + 300], kv, kv, page, seed=1)
+    at = [n_pages - 1 - 7 * i for i in range(c.table.shape[1])]
+    for j, p in enumerate(at):
+        k[p], v[p] = c.k[c.table[0, j]], c.v[c.table[0, j]]
+    c.table[0, :], c.k, c.v = at, k, v
+    # the last rows once more, by append
+    last = torch.cat([c.q.reshape(new, -1), torch.randn(new, 2 * kv * 64, device="cuda").to(dt)], 1)[:, None]
+    pos = np.arange(300, new + 300)
+    slots = np.array(at)[pos // page] * page + pos % page
+    cache_append(last, ints(pos), ints(slots), k, v, kv, kv, freqs=None, q=c.q)
+    assert torch.equal(k[int(slots[-1]) // page, :, int(slots[-1]) % page].reshape(-1), last[-1, 0, kv * 64:2 * kv * 64])
+    out = c.run()
+    c.k, c.v, c.table = k[at], v[at], np.arange(len(at))[None]
+    del k, v
+    c.check()
+    assert torch.equal(c.run(), out)
+
+
+def test_two_streams_at_once(cuda_device):
+    """Calls that overlap on two streams, of every kernel, each with its own workspace: the same bits as alone."""
+    cases = [Case("fp16", n, t, 8, 4, 64, seed=i) for i, (n, t) in enumerate(
+        [([1, 2], [3000, 700]), ([40, 1], [2000, 2000]), ([200, 20], [1500, 900])])]
+    want = [c.run().clone() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(6):
+        for i, c in enumerate(cases):
+            for s in streams:
+                with torch.cuda.stream(s):
+                    got.append((i, c.run()))
+    torch.cuda.synchronize()
+    for i, g in got:
+        assert torch.equal(g, want[i])
+
+
+@pytest.mark.parametrize("new", [1, 50, 300])
+def test_captured_attention_follows_the_lengths(cuda_device, new):
+    """A captured call reads lengths and tables at replay: shorter, longer and empty pushes within its capacity."""
+    c = Case("fp16", [new, new], [new + 800, new + 500], 4, 2, 32, gates=True)
+    table, cu, total = ints(c.table), ints(c.cu), ints(c.total)
+    out, status = torch.zeros_like(c.q), ints([0])
+    call = lambda: cache_attention(c.q, c.k, c.v, table, cu, total, c.max_new, c.max_total, gates=c.gates, out=out,  # noqa: E731
+                                   status=status)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for a, b in ([new, new], [0, new], [new, 0], [0, 0], [(new + 1) // 2, 1]):
+        c.new, c.cu = [a, b], np.array([0, a, a + b])
+        cu.copy_(ints(c.cu))
+        out.fill_(3.0)
+        graph.replay()
+        assert status.item() == 0 and (out[a + b:] == 3.0).all()
+        want = torch.full_like(out, 3.0)
+        c.run(want)
+        assert torch.equal(out, want)
+
+
 # ------------------------------------------------------------------------------------------------ together
 def test_whole_chunk_equals_the_chunk_stages(tiny_cuda, tiny_cfg):
     """A whole chunk pushed into an empty cache: the same attention as trc_rope_pack + trc_attention (time mode)."""

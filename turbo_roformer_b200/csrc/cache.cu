@@ -344,14 +344,14 @@ int sm_count() {
   return n;
 }
 
-// Which kernel takes a sequence, by its rows per cache head (new frames x query heads that share it). Measured with
-// 496 heads over 1,700 frames (us; HBM floor 34-43 us):
-//   rows                        16   20   28   40   64  128  200  256  384
-//   cache_rows_kernel           ROWS_FIGURES
-//   cache_tiles_kernel          SEPARATE_FIGURES
-//   cache_tiles_kernel, shared  SHARED_FIGURES
-constexpr int kFewRows = 32;      // cache_rows_kernel
-constexpr int kSeparateRows = 256;  // cache_tiles_kernel with separate tiles; above it with shared ones
+// Which kernel takes a sequence, by its rows per cache head (new frames x query heads that share it). A call's time
+// with 496 heads over 1,700 frames, us (HBM floor 33 us for one row, 38 us for 128; tensor floor 60 us for 384):
+//   rows                         1   16   20   32   40   64  128  200  256  384  768
+//   cache_rows_kernel           45   50   57   61
+//   cache_tiles_kernel                    79   80   82   84   93  143  152  206  464
+//   cache_tiles_kernel, shared           104  106  107  108  116  139  146  178  362
+constexpr int kFewRows = 32;        // cache_rows_kernel
+constexpr int kSeparateRows = 128;  // cache_tiles_kernel with separate tiles; above it with shared ones
 constexpr int kCtasPerSm = 2;     // of cache_rows_kernel
 
 // The launches of a call and where their parts go in the workspace.

@@ -9,8 +9,9 @@
 //     one channel, one producer. Tiles have key ranges of their own within the run (causal, window): a tile takes part
 //     in the steps of its range and only releases the others.
 //   * Otherwise each tile is a channel of its own, a worker with its own share of the line, items of one tile and own
-//     stages. Pushes of up to 256 rows keep all three tiles busy this way, where the shared form would leave one or
-//     two idle; longer ones are faster shared, which loads a third of the key bytes.
+//     stages. Pushes of up to 128 rows keep all three tiles busy this way, where the shared form would leave two idle
+//     (128 rows of 496 heads over 1,700 frames: 93 against 116 us); longer ones are faster shared, which loads a
+//     third of the key bytes and has 152 instead of 128 registers for a softmax thread (384 rows: 178 against 206 us).
 //   * Producers and MMA issuers are warps of their own: issuing a step's products alone takes a thread 450 cycles or
 //     more (the tensor pipe is shared by the three), and a step lasts about 2,600. Keys and values have stages of
 //     their own, K freed by S, V by P V.
