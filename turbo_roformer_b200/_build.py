@@ -1,4 +1,4 @@
-"""Build libtrcuda.so in-tree with nvcc for sm_100a (B200).
+"""Build libtrcuda.so in-tree with nvcc for sm_100a (B200), and the frame cache's Python binding.
 
 ``python -m turbo_roformer_b200._build`` or ``build()``; the library lands next to this file so that it
 travels with the source tree. nvcc cross-compiles: no GPU is needed to build.
@@ -74,5 +74,56 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB_PATH
 
 
+BINDING_SOURCE = os.path.join(CSRC, "cache_binding.cpp")
+BINDING_PATH = os.path.join(HERE, "_cache_binding.so")
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile the frame cache's Python binding (host code against torch's headers; skipped when up to date)."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    with open(BINDING_SOURCE, "rb") as f:
+        digest = hashlib.sha256(f.read() + f"{torch.__version__} {sys.version}".encode()).hexdigest()[:16]
+    stamp = BINDING_PATH + ".hash"
+    if not force and os.path.exists(BINDING_PATH) and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read().strip() == digest:
+                return BINDING_PATH
+    cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
+    lib = os.path.join(root, "lib")
+    cmd = [
+        os.environ.get("CXX") or shutil.which("g++") or "c++",
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        *(f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"), cuda,
+                             sysconfig.get_paths()["include"])),
+        BINDING_SOURCE,
+        "-o",
+        BINDING_PATH + ".tmp",
+        f"-L{lib}",
+        "-ltorch_python",
+        "-ltorch_cpu",
+        "-lc10",
+        "-lc10_cuda",
+        f"-Wl,-rpath,{lib}",
+    ]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    os.replace(BINDING_PATH + ".tmp", BINDING_PATH)
+    with open(stamp, "w") as f:
+        f.write(digest + "\n")
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
+    print(build_binding(force="--force" in sys.argv, verbose=True))
     print(build(force="--force" in sys.argv, verbose=True))
