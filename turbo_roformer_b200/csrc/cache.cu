@@ -74,10 +74,11 @@ struct PlanArgs {
   int n_seqs, page_log2, n_free, table_stride, capacity;
 };
 
-constexpr int kPlanThreads = 512;
+constexpr int kPlanThreads = 1024;
 
-__device__ __forceinline__ int pages_of(int64_t frames, int page_log2) {
-  return (int)((frames + (1 << page_log2) - 1) >> page_log2);
+// frames <= 2^30
+__device__ __forceinline__ int pages_of(int frames, int page_log2) {
+  return (frames + (1 << page_log2) - 1) >> page_log2;
 }
 
 // last x in [0, n) with v[x] <= at, for ascending v with v[0] <= at
@@ -110,17 +111,14 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     }
     cached[r] = c;
     cu[r] = n;
-    if (blockIdx.x == 0) {
-      a.total[r] = c + n;
-      if (pages_of((int64_t)c + n, a.page_log2) > a.table_stride) bad |= TRC_CACHE_TABLE_FULL;
-    }
+    if (pages_of(c + n, a.page_log2) > a.table_stride) bad |= TRC_CACHE_TABLE_FULL;
   }
   __syncthreads();
   // an odd number of sequences per thread: neighbours' strides then miss each other's banks
   const int per = ((a.n_seqs + kPlanThreads - 1) / kPlanThreads) | 1;
   const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
   int64_t rows = 0, pages = 0;
-  auto pages_for = [&](int c, int n) { return pages_of((int64_t)c + n, a.page_log2) - pages_of(c, a.page_log2); };
+  auto pages_for = [&](int c, int n) { return pages_of(c + n, a.page_log2) - pages_of(c, a.page_log2); };
   for (int r = r0; r < r1; ++r) {
     rows += cu[r];
     pages += pages_for(cached[r], cu[r]);
@@ -140,18 +138,20 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     part[1][warp] = ps;
   }
   __syncthreads();
-  rs -= rows;
-  ps -= pages;
-  int64_t all_rows = 0, all_pages = 0;
+  static_assert(kPlanThreads == 1024, "one warp scans the warps' sums");
+  if (warp < 2) {
+    int64_t x = part[warp][lane];
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) {
-      rs += part[0][w];
-      ps += part[1][w];
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
     }
-    all_rows += part[0][w];
-    all_pages += part[1][w];
+    part[warp][lane] = x;
   }
+  __syncthreads();
+  rs += (warp ? part[0][warp - 1] : 0) - rows;
+  ps += (warp ? part[1][warp - 1] : 0) - pages;
+  const int64_t all_rows = part[0][31], all_pages = part[1][31];
   for (int r = r0; r < r1; ++r) {
     const int n = cu[r];
     cu[r] = (int)min(rs, (int64_t)INT_MAX);
@@ -170,15 +170,18 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     if (bad) atomicOr(&flags, bad);
   }
   __syncthreads();
-  if (blockIdx.x == 0) {
-    for (int r = threadIdx.x; r <= a.n_seqs; r += kPlanThreads) a.cu[r] = cu[r];
-    if (threadIdx.x == 0) {
-      a.counts[0] = min(live_pages, a.n_free);
-      a.counts[1] = flags;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.counts[0] = min(live_pages, a.n_free);
+    a.counts[1] = flags;
+  }
+  const int stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + threadIdx.x;
+  for (int r = first; r <= a.n_seqs; r += stride) {
+    a.cu[r] = cu[r];
+    if (r < a.n_seqs) {
+      const int c = a.cached[r], n = a.fresh[r];  // as above: bad lengths count as none
+      a.total[r] = c < 0 || n < 0 || (int64_t)c + n > (1 << 30) ? 0 : c + n;
     }
   }
-
-  const int stride = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + threadIdx.x;
   // fresh pages into the table
   for (int64_t e = first; e < live_pages; e += stride) {
     const int r = last_upto(base, a.n_seqs, (int)e);
@@ -524,7 +527,7 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
   // a thread for every four rows
   const int64_t most = (int64_t)max_rows / 4 + 1;
   const int blocks = (int)((most + trc::kPlanThreads - 1) / trc::kPlanThreads);
-  return trc::launch("cache plan", trc::cache_plan_kernel, dim3(blocks < 2 * sms ? blocks : 2 * sms), trc::kPlanThreads,
+  return trc::launch("cache plan", trc::cache_plan_kernel, dim3(blocks < sms ? blocks : sms), trc::kPlanThreads,
                      smem, (cudaStream_t)stream, a);
 }
 
