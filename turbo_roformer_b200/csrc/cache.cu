@@ -64,7 +64,8 @@ int page_log2_of(int page) {
 // flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows, four at a time (one
 // search, then onwards; vector stores). Nothing is exchanged between blocks, so one launch serves any batch: a row's
 // page is either fresh (read from the free list, not from the table that another block is writing) or was in the table
-// before. Lengths and sums sit in shared memory; the scan is a latency of some 3 us and bounds small batches.
+// before. Lengths and sums sit in shared memory. Bound by the latency of the scan: a push of 8 streams takes 4 us, one
+// of 4,001 sequences and a million rows 11 to 15 us (8.9 MB: 1.4 us of HBM).
 struct PlanArgs {
   const int32_t* cached;
   const int32_t* fresh;  // new lengths
@@ -234,6 +235,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
 //   * its four angles (position x frequency in fp64, reduced to half turns, because fp32 loses the angle of far
 //     positions) are computed once, while its first loads travel, and stay in registers for all its heads;
 //   * the 128-byte rows that a head's frames write to a page lie one behind the other.
+// 1,700 frames of 62 bands x 24 head rows with gates (653 MB): 115 us, 5.7 TB/s, 0.87 of the copy rate; one thread per
+// vector of a flat run, the angles in shared memory, took 187 us (184 instructions per vector).
 constexpr int kAppendThreads = 256;
 constexpr int kAppendFlight = 4;  // head rows per thread in flight
 constexpr int kAppendFrames = 16;

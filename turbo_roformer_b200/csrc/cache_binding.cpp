@@ -2,8 +2,8 @@
 // libtrcuda's C ABI (include/trcuda.h), as one extension module.
 //
 // A push of a few frames takes three calls whose kernels run 3 to 6 us. Reading shapes, types, devices and strides of
-// up to nine tensors through Python attributes, and some twenty arguments through ctypes, took 11 to 15 us per call;
-// the same here takes PYTHON_CALL_FIGURES. The library itself stays free of torch types: the module gets the
+// up to nine tensors through Python attributes, and some twenty arguments through ctypes, took 11 to 16 us per call;
+// the same here takes 4 to 8 us, the launches included. The library itself stays free of torch types: the module gets the
 // addresses of its entry points from the ctypes binding (bind).
 #include <Python.h>
 
