@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegsIssue) : "memory");
     else
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kRegsLoad) : "memory");
-    if (warp < kCtTiles && lane == 0) {
+    if (warp < kCtTiles) {
       // ------------------------------------------------------------------ MMA issuer of tile x
       const int x = warp, c = SHARED ? 0 : x;
       const CacheRun* runs = reinterpret_cast<const CacheRun*>(smem + S::kRun) + c * kCtRuns;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       uint32_t kp = 0, vp = 0;   // and their phases
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity, args.status, kErrWaitMma, abort_flag)) ok = false;
+        if (ok && !mbar_wait_warp(bar, parity, args.status, kErrWaitMma, abort_flag)) ok = false;
         return ok;
       };
       auto next_stage = [&](int& st, uint32_t& phase) {
@@ -254,10 +254,10 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
       auto pass = [&](int steps) {  // steps of other tiles' keys: released once filled
         for (; steps > 0 && ok; --steps) {
           if (!wait(&kf[ks], kp)) return;
-          mbar_arrive(&ke[ks]);
+          if (lane == 0) mbar_arrive(&ke[ks]);
           next_stage(ks, kp);
           if (!wait(&vf[vs], vp)) return;
-          mbar_arrive(&ve[vs]);
+          if (lane == 0) mbar_arrive(&ve[vs]);
           next_stage(vs, vp);
         }
       };
@@ -267,11 +267,14 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         tc_fence_after();
         const uint64_t qd = q_desc0 + (uint64_t)(qb * (kCtTiles * S::kTileQ >> 4));
         const uint64_t kd = k_desc + (uint64_t)(ks * (S::kTileKV >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tS, qd + 2 * kk, kd + 2 * kk, idesc_qk, kk > 0 ? 1u : 0u);
-        mma_commit(&s_full[x]);
-        mma_commit(&ke[ks]);
-        if (last) mma_commit(&q_empty[c * kBufs + qb]);
+          for (int kk = 0; kk < 4; ++kk) mma_f16_ss(tS, qd + 2 * kk, kd + 2 * kk, idesc_qk, kk > 0 ? 1u : 0u);
+          mma_commit(&s_full[x]);
+          mma_commit(&ke[ks]);
+          if (last) mma_commit(&q_empty[c * kBufs + qb]);
+        }
+        __syncwarp();
         next_stage(ks, kp);
       };
       for (int r = 0; ok; ++r) {
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         const int after = run.a1 - e;
         if (SHARED) {
           pass(b - run.a0);
-          if (b == e) mbar_arrive(&q_empty[c * kBufs + qb]);
+          if (b == e && lane == 0) mbar_arrive(&q_empty[c * kBufs + qb]);
         }
         if (b < e) {
           issue_s(e - b == 1);  // the softmax warps have taken S(n - 1): waited for below
@@ -295,18 +298,23 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
             if (j == b && active > 0 && !wait(&o_free[x], (active - 1) & 1)) break;
             tc_fence_after();
             const uint64_t vd = v_desc + (uint64_t)(vs * (S::kTileKV >> 4));
+            if (elect_one()) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_f16_ts(tO, tP + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (j > b || kk > 0) ? 1u : 0u);
-            mma_commit(&p_free[x]);
-            mma_commit(&ve[vs]);
+              for (int kk = 0; kk < 4; ++kk)
+                mma_f16_ts(tO, tP + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (j > b || kk > 0) ? 1u : 0u);
+              mma_commit(&p_free[x]);
+              mma_commit(&ve[vs]);
+            }
+            __syncwarp();
             next_stage(vs, vp);
           }
           ++active;
         }
         if (SHARED) pass(after);
       }
-      mma_commit(&drain[x]);
+      __syncwarp();
+      if (elect_one()) mma_commit(&drain[x]);
+      __syncwarp();
       const uint64_t t0 = global_ns();
       while (!mbar_try_wait(&drain[x], 0) && global_ns() - t0 < kWaitLimitNs) {
       }
@@ -582,7 +590,8 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           for (int k = 0; k < 32; k += 2) {
             const int at = c * 32 + k;
             const float2 xv = __ffma2_rn(make_float2(sc[at], sc[at + 1]), scale2, shift2);
-            const float2 pv = (k & 7) == 6 ? ex2_poly2(xv) : make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
+            // one pair in eight on the FMA pipe: the polynomial costs instructions, and one in four lost 1.5 %
+            const float2 pv = (k & 15) == 14 ? ex2_poly2(xv) : make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
             l2 = __fadd2_rn(l2, pv);
             packed[k >> 1] = OperandType<TIn>::pack2(pv.x, pv.y);
           }
