@@ -11,7 +11,7 @@
 //   * Otherwise each tile is a channel of its own, a worker with its own share of the line, items of one tile and own
 //     stages. Pushes of up to 128 rows keep all three tiles busy this way, where the shared form would leave two idle
 //     (128 rows of 496 heads over 1,700 frames: 93 against 116 us); longer ones are faster shared, which loads a
-//     third of the key bytes and has 152 instead of 128 registers for a softmax thread (384 rows: 178 against 206 us).
+//     third of the key bytes (384 rows: 178 against 206 us).
 //   * Producers and MMA issuers are warps of their own: issuing a step's products alone takes a thread 450 cycles or
 //     more (the tensor pipe is shared by the three), and a step lasts about 2,600. Keys and values have stages of
 //     their own, K freed by S, V by P V.
@@ -64,14 +64,15 @@ struct CtSmem {
   static constexpr int kScan = kBar + 768 + 256;
   static constexpr int bytes(int n_seqs) { return kScan + (n_seqs + 1) * 8 + 1024; }
   // Warps 0-2 issue; the producers are warp 3 (shared) or warps 4-6; then twelve softmax warps. Registers per thread
-  // after setmaxnreg add up to what the launch gives (checked before it): 512 x 128 = 128 x 56 + 384 x 152, or
-  // 640 x 96 = 128 x 40 + 128 x 56 + 384 x 128.
+  // after setmaxnreg add up to what the launch gives (checked before it): 512 x 128 = 128 x 80 + 384 x 144, or
+  // 640 x 96 = 128 x 72 + 128 x 72 + 384 x 112. The issuers and producers need theirs: with 40 and 56 (128 for the
+  // softmax) they spill inside their loops, and 100 rows over 1,700 frames take 138 instead of 129 us.
   static constexpr int kProducer0 = SHARED ? 3 : 4;
   static constexpr int kSoftmax0 = SHARED ? 4 : 8;
   static constexpr int kThreads = 32 * (kSoftmax0 + 4 * kCtTiles);
-  static constexpr int kRegsIssue = SHARED ? 56 : 40;
-  static constexpr int kRegsLoad = 56;
-  static constexpr int kRegsSoftmax = SHARED ? 152 : 128;
+  static constexpr int kRegsIssue = SHARED ? 80 : 72;
+  static constexpr int kRegsLoad = 72;
+  static constexpr int kRegsSoftmax = SHARED ? 144 : 112;
   static constexpr int kRegs = 128 * (kRegsIssue + (SHARED ? 0 : kRegsLoad) + 3 * kRegsSoftmax);
   static_assert(kBar % 8 == 0 && kScan % 8 == 0, "alignment");
   static_assert(kScan + (kCacheMaxSeqs + 1) * 8 + 1024 <= 232448, "shared memory per CTA");
