@@ -353,11 +353,11 @@ int sm_count() {
 // Which kernel takes a sequence, by its rows per cache head (new frames x query heads that share it). A call's time
 // with 496 heads over 1,700 frames, us (HBM floor 33 us for one row, 38 us for 128; tensor floor 60 us for 384):
 //   rows                         1   16   20   32   40   64  128  200  256  384  768
-//   cache_rows_kernel           45   50   57   61
-//   cache_tiles_kernel                    79   80   82   84   93  143  152  206  464
-//   cache_tiles_kernel, shared           104  106  107  108  116  139  146  178  362
+//   cache_rows_kernel           45   49   56   59
+//   cache_tiles_kernel                    68   68   70   70   75  120  126  176  326
+//   cache_tiles_kernel, shared            95   96   96   97  100  128  136  158  293
 constexpr int kFewRows = 32;        // cache_rows_kernel
-constexpr int kSeparateRows = 128;  // cache_tiles_kernel with separate tiles; above it with shared ones
+constexpr int kSeparateRows = 256;  // cache_tiles_kernel with separate tiles; above it with shared ones
 constexpr int kCtasPerSm = 2;     // of cache_rows_kernel
 
 // The launches of a call and where their parts go in the workspace.
