@@ -9,19 +9,22 @@
 //     one channel, one producer. Tiles have key ranges of their own within the run (causal, window): a tile takes part
 //     in the steps of its range and only releases the others.
 //   * Otherwise each tile is a channel of its own, a worker with its own share of the line, items of one tile and own
-//     stages. Pushes of up to 128 rows keep all three tiles busy this way, where the shared form would leave two idle
-//     (128 rows of 496 heads over 1,700 frames: 93 against 116 us); longer ones are faster shared, which loads a
-//     third of the key bytes (384 rows: 178 against 206 us).
-//   * Producers and MMA issuers are warps of their own: issuing a step's products alone takes a thread 450 cycles or
-//     more (the tensor pipe is shared by the three), and a step lasts about 2,600. Keys and values have stages of
-//     their own, K freed by S, V by P V.
+//     stages. Pushes of up to 256 rows keep all three tiles busy this way, where the shared form would leave one or two
+//     idle (128 rows of 496 heads over 1,700 frames: 75 against 100 us, 256: 126 against 136); longer ones are faster
+//     shared, which loads a third of the key bytes (384 rows: 158 against 176 us).
+//   * Producers and MMA issuers are warps of their own: issuing a step's products takes 750 cycles of its 2,400 (the
+//     tensor pipe is shared by the three). Issuers stay whole warps and elect a lane for the MMAs and commits (5 % over
+//     a single lane that runs the whole role). Keys and values have stages of their own, K
+//     freed by S, V by P V.
 //   * V rows outside the item's keys (behind the sequence's end, before the window) are zeroed in shared memory by the
 //     producer before it hands the stage on, because pages hold anything there and 0 x NaN is NaN; scores are replaced
 //     per row, behind one vote per step.
 //   * A run that is not a whole item leaves its rows' sums, maxima and weights in the workspace for the join.
-// Measured: a step of three shared tiles takes 1.13 us and of three separate ones 1.4 us (the time attention: 1.19), a
-// run's start and end 3.6 and 5 us, a launch 12 us up to its first weights. 1,701 frames x 496 heads: 610 us (600
-// TFLOP/s) on a cool GPU, 685 us under the power cap. The softmax warps' instructions bound it, as in the time attention.
+// Measured: a step of three shared tiles takes 2,400 cycles and of three separate ones 3,300 to 3,600, a run's start
+// and end about three steps, a launch 12 us up to its first weights. 1,701 frames x 496 heads: 650 to 680 us under the
+// power cap. A step's time is neither the exponentials' nor the products' alone: without any exponential it is a fifth
+// less, with a quarter of the products the same. It is the chain from S to P to the next product, of which three tiles
+// hide a part (384 rows: issue slots 52 % used, tensor pipe 32 %, MUFU 58 %).
 // Roles: warps 0-2 MMA issuers of tiles 0-2, warp 3 owns TMEM, producers, softmax + epilogue (CtSmem).
 #pragma once
 
@@ -55,7 +58,7 @@ struct CtSmem {
   static constexpr int kTileQ = 128 * 64 * 2;
   static constexpr int kTileKV = 64 * 64 * 2;
   static constexpr int kQ = 0;                                                          // [bufs][tiles]
-  static constexpr int kKV = kQ + kQBufs * kCtTiles * kTileQ;                                    // [channels][K, V][stages]
+  static constexpr int kKV = kQ + kQBufs * kCtTiles * kTileQ;                              // [channels][K, V][stages]
   static constexpr int kScale = kKV + kChannels * 2 * kStages * kTileKV;                // [tiles][128] fp32
   static constexpr int kOut = kScale + kCtTiles * 128 * 4;                              // [softmax warps][8 rows]
   static constexpr int kRun = kOut + 4 * kCtTiles * 1024;                               // [channels][kCtRuns]
@@ -79,7 +82,7 @@ struct CtSmem {
 };
 
 // A warp's rows of O from TMEM to where they go (thread = row, dst null: nowhere), and the accumulator's release. A
-// function of its own, because inlined into the softmax loop its registers cost every step (1.36 instead of 1.15 us).
+// function of its own, because inlined into the softmax loop its registers cost every step a fifth.
 template <typename TIn, int ROWS>
 __device__ __noinline__ void ct_finish(uint32_t t_o, void* dst, bool is_part, float scale, uint8_t* stage,
                                        uint64_t* o_free) {

@@ -258,8 +258,7 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
-// True in one lane of a converged warp, the same one every time. Instructions of one thread (MMAs, commits) inside
-// `if (elect_one())` keep their operands in uniform registers.
+// True in one lane of a converged warp, the same one every time: the lane that issues MMAs and commits.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
   asm volatile(
