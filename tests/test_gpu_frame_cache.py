@@ -466,6 +466,47 @@ def test_attention_shared_pages(cuda_device):
     c.check()
 
 
+@pytest.mark.parametrize("rows", [250, 255, 256, 257, 260, 512, 513])
+def test_attention_row_counts_around_shared_tiles(cuda_device, rows):
+    """The border between separate and shared tiles, with a sequence of every other variant in the same batch."""
+    c = Case("bf16", [rows, 3, 0, rows // 2, 40], [rows + 130, 200, 90, rows, 41], 2, 2, 64, gates=True, seed=rows)
+    c.check(causal=True)
+    c.check(causal=False, window=90)
+
+
+@pytest.mark.parametrize("new", [300, 700])
+def test_attention_shared_tiles_keep_the_rules(cuda_device, new):
+    """Rows that see nothing, NaN queries, pages given back and bad pages in pushes whose tiles share their keys."""
+    test_attention_rows_that_see_nothing(cuda_device, new)
+    test_attention_pages_before_the_window_are_not_read(cuda_device, new)
+    test_attention_bad_lengths_and_pages(cuda_device, new)
+    c = Case("fp16", [new], [new + 100], 2, 2, 16)
+    want = c.run().clone()
+    c.q[1, 0, 5] = float("nan")
+    got = c.run()
+    assert got[1, 0].isnan().all()
+    want[1, 0] = got[1, 0] = 0
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [400])
+def test_shared_tiles_on_streams_and_divided(cuda_device, new):
+    test_attention_on_another_stream_and_repeated(cuda_device, new)
+    test_pool_offsets_past_32_bits(cuda_device, new)
+    cases = [Case("fp16", n, t, 8, 4, 64, seed=i) for i, (n, t) in enumerate([([200, 20], [1500, 900]), ([1], [3000])])]
+    want = [c.run().clone() for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = []
+    for _ in range(4):
+        for c, st in zip(cases, streams):
+            with torch.cuda.stream(st):
+                got.append(c.run())
+    torch.cuda.synchronize()
+    for k, out in enumerate(got):
+        assert torch.equal(out, want[k % 2])
+
+
 @pytest.mark.parametrize("new", [2, 60, 200])
 def test_pool_offsets_past_32_bits(cuda_device, new):
     """Pages whose elements lie more than 2^31 (and bytes more than 2^32) into the pool, written and read."""

@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           for (int k = 0; k < 32; k += 2) {
             const int at = c * 32 + k;
             const float2 xv = __ffma2_rn(make_float2(sc[at], sc[at + 1]), scale2, shift2);
-            // one pair in eight on the FMA pipe: the polynomial costs instructions, and one in four lost 1.5 %
+            // one pair in eight on the FMA pipe (one in four: 1.5 % slower, as its instructions cost more than they relieve)
             const float2 pv = (k & 15) == 14 ? ex2_poly2(xv) : make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
             l2 = __fadd2_rn(l2, pv);
             packed[k >> 1] = OperandType<TIn>::pack2(pv.x, pv.y);
