@@ -205,9 +205,9 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
  * [n_rows][heads][64] with q_stride / out_stride elements between rows; d_gates [n_rows][heads] fp32 or NULL.
  * max_new and max_total: the longest new part and the longest total, as far as the host knows them; they choose
  * between variants and never change which rows and keys are computed. d_workspace is not used where
- * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are finite; what the
- * pages hold behind `total`, or wholly before every row's window, is not read into any result. d_out does not overlap
- * d_q. */
+ * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are
+ * finite; what the pages hold behind `total`, or wholly before every row's window, is not read into any result. d_out
+ * does not overlap d_q. */
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
                         const int32_t* d_table, int table_stride, const int32_t* d_cu, const int32_t* d_total,
                         int n_seqs, int n_rows, int max_new, int max_total, int heads, int kv_heads, int page,

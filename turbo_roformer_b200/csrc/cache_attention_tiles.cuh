@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           request(map_v, dst, &raw[c], y);
           if (!wait(&raw[c], (uint32_t)raws++ & 1)) return;
           // 16-byte chunks; the swizzle stays within a row
-          for (int k = lane; k < (lo - key0) * 8; k += 32) *reinterpret_cast<uint4*>(dst + k * 16) = make_uint4(0, 0, 0, 0);
+          for (int k = lane; k < (lo - key0) * 8; k += 32)
+            *reinterpret_cast<uint4*>(dst + k * 16) = make_uint4(0, 0, 0, 0);
           for (int k = max(hi - key0, 0) * 8 + lane; k < kCacheStep * 8; k += 32)
             *reinterpret_cast<uint4*>(dst + k * 16) = make_uint4(0, 0, 0, 0);
           fence_async_smem();
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           for (int k = 0; k < 32; k += 2) {
             const int at = c * 32 + k;
             const float2 xv = __ffma2_rn(make_float2(sc[at], sc[at + 1]), scale2, shift2);
-            // one pair in eight on the FMA pipe (one in four: 1.5 % slower, as its instructions cost more than they relieve)
+            // one pair in eight on the FMA pipe; one in four is 1.5 % slower, the polynomial being more instructions
             const float2 pv = (k & 15) == 14 ? ex2_poly2(xv) : make_float2(ex2_approx(xv.x), ex2_approx(xv.y));
             l2 = __fadd2_rn(l2, pv);
             packed[k >> 1] = OperandType<TIn>::pack2(pv.x, pv.y);
