@@ -204,7 +204,8 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
  * window > 0: j > the row's frame - window (0: no limit). A row without keys is zero. d_q and d_out
  * [n_rows][heads][64] with q_stride / out_stride elements between rows; d_gates [n_rows][heads] fp32 or NULL.
  * max_new and max_total: the longest new part and the longest total, as far as the host knows them; they choose
- * between variants and never change which rows and keys are computed. d_workspace is not used where
+ * between variants and never change which rows and keys are computed. A score of NaN or +inf that a row sees makes the
+ * row NaN; one of -inf weighs nothing (a row of such scores only is zero). d_workspace is not used where
  * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are
  * finite; what the pages hold behind `total`, or wholly before every row's window, is not read into any result. d_out
  * does not overlap d_q. */

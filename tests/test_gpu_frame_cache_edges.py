@@ -1,0 +1,72 @@
+"""The frame cache on the GPU where it can go wrong: blocks of several frames, keys and values that are not finite,
+lengths that do not fit, buffers that overlap. Tolerances are those derived in test_gpu_frame_cache.py."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import cache_oracle as CO
+from turbo_roformer_b200 import cache_append, cache_attention, cache_plan
+
+from .test_gpu_frame_cache import FREQS, Case, f64, ints, test_append_matches_oracle as check_append
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ not finite
+VARIANTS = [1, 20, 60, 140, 400]  # new frames of one query head: every kernel form
+
+
+def put(c, pool, frame, value, dims=slice(None)):
+    """`value` into a frame of the first sequence, all cache heads."""
+    pool[int(c.table[0, frame // c.page]), :, frame % c.page, dims] = value
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", VARIANTS)
+def test_nan_key_makes_the_rows_that_see_it_nan(cuda_device, dtype, new):
+    """A NaN in one key, at every place of 16: rows that see it are NaN, the others as if it were not there."""
+    c = Case(dtype, [new], [new + 70], 2, 2, 32)
+    want = c.run().clone()
+    keep = c.k.clone()
+    for at in [*range(16, 32), 70 + new // 2, 70 + new - 1]:
+        c.k.copy_(keep)
+        put(c, c.k, at, float("nan"), slice(5, 6))
+        got = c.run()
+        sees = torch.arange(70, 70 + new, device="cuda") >= at
+        assert got[sees].isnan().all(), at
+        assert torch.equal(got[~sees], want[~sees]), at
+
+
+@pytest.mark.parametrize("new", VARIANTS)
+def test_nan_key_alone_in_the_window(cuda_device, new):
+    """Rows that see one key only: NaN where that key is NaN, the value itself elsewhere."""
+    c = Case("fp16", [new], [new + 33], 2, 2, 16)
+    want = c.run(window=1).clone()
+    for frame in range(33, 33 + new, 3):
+        put(c, c.k, frame, float("nan"))
+    got = c.run(window=1)
+    gone = torch.arange(new, device="cuda") % 3 == 0
+    assert got[gone].isnan().all() and torch.equal(got[~gone], want[~gone])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", VARIANTS)
+def test_infinite_keys(cuda_device, dtype, new):
+    """A key element of +inf: scores of +inf make the row NaN, scores of -inf are weights of zero."""
+    for at in (3, 14, 15, 65, 78, 79):
+        c = Case(dtype, [new], [new + 100], 1, 1, 64)
+        put(c, c.k, at, float("inf"), slice(9, 10))
+        got = f64(c.run(causal=False))
+        up = f64(c.q)[:, 0, 9] > 0
+        assert np.isnan(got[up]).all(), at
+        k, v = np.nan_to_num(f64(c.k), posinf=1e30), np.nan_to_num(f64(c.v))
+        ref, size, keys = CO.attention(f64(c.q), k, v, c.table, c.cu, c.total, c.page, False, 0, 0.125)
+        u = torch.finfo(c.dtype).eps / 2
+        norms = np.linalg.norm(f64(c.q)[:, 0], axis=-1).max() * np.linalg.norm(np.where(k < 1e30, k, 0), axis=-1).max()
+        e = 7.5e-5 + 70 * 2.0**-24 * norms * 0.125
+        tol = 1.01 * (u * np.abs(ref) + size * (u + 2 * e + 2 * (new + 100) * 2.0**-24)) + 2.0**-24
+        tol = tol + (new + 100) * 2.0**-25 * np.abs(v).max() * (c.dtype == torch.float16)
+        assert (np.abs(got - ref)[~up] <= tol[~up]).all(), at

@@ -562,28 +562,30 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
           for (int k = 0; k < 64; ++k)
             if (k >= kmax || k < kmin) sc[k] = -INFINITY;
         }
+        // A visible score of NaN or +inf makes the row NaN, through its maximum: the polynomial would lose a NaN.
         float mx4[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
         for (int k = 4; k < 60; k += 8) {
-          mx4[0] = fmax3(mx4[0], sc[k], sc[k + 4]);
-          mx4[1] = fmax3(mx4[1], sc[k + 1], sc[k + 5]);
-          mx4[2] = fmax3(mx4[2], sc[k + 2], sc[k + 6]);
-          mx4[3] = fmax3(mx4[3], sc[k + 3], sc[k + 7]);
+          mx4[0] = fmax3_nan(mx4[0], sc[k], sc[k + 4]);
+          mx4[1] = fmax3_nan(mx4[1], sc[k + 1], sc[k + 5]);
+          mx4[2] = fmax3_nan(mx4[2], sc[k + 2], sc[k + 6]);
+          mx4[3] = fmax3_nan(mx4[3], sc[k + 3], sc[k + 7]);
         }
-        const float m_tile =
-            fmaxf(fmax3(mx4[0], mx4[1], sc[60]), fmax3(mx4[2], mx4[3], fmax3(sc[61], sc[62], sc[63]))) *
-            args.scale_log2;
+        const float m_tile = fmax3_nan(fmax3_nan(mx4[0], mx4[1], sc[60]), fmax3_nan(mx4[2], mx4[3], sc[61]),
+                                       fmax3_nan(sc[62], sc[63], sc[63])) *
+                             args.scale_log2;
         bool rescale = false;
         float alpha = 1.0f;
         if (j == b) {
-          m_run = m_tile;
+          m_run = m_tile < INFINITY ? m_tile : NAN;
         } else {
           // from -inf (no visible key so far): O and the weight are zero, 2^-inf = 0 keeps them
-          const bool need = m_tile > m_run + kRescaleThreshold;
+          const bool need = live && !(m_tile <= m_run + kRescaleThreshold);
           rescale = __any_sync(0xffffffffu, need);
           if (need) {
-            alpha = ex2_approx(m_run - m_tile);
-            m_run = m_tile;
+            const float m_next = m_tile < INFINITY ? m_tile : NAN;
+            alpha = ex2_approx(m_run - m_next);
+            m_run = m_next;
           }
         }
         const float shift = m_run == -INFINITY ? 0.f : -m_run;
