@@ -70,3 +70,20 @@ def test_infinite_keys(cuda_device, dtype, new):
         tol = 1.01 * (u * np.abs(ref) + size * (u + 2 * e + 2 * (new + 100) * 2.0**-24)) + 2.0**-24
         tol = tol + (new + 100) * 2.0**-25 * np.abs(v).max() * (c.dtype == torch.float16)
         assert (np.abs(got - ref)[~up] <= tol[~up]).all(), at
+
+
+@pytest.mark.parametrize("dtype,big", [("bf16", 3e38), ("fp16", 65504.0)])
+@pytest.mark.parametrize("new", VARIANTS)
+def test_hidden_values_of_any_finite_size(cuda_device, dtype, big, new):
+    """Values of frames that a row's masks hide do not reach it, the type's largest among them."""
+    c = Case(dtype, [new], [new + 40], 2, 2, 16)
+    c.v.nan_to_num_(0.0)
+    c.v.mul_(2.0**-40 if dtype == "bf16" else 1.0)
+    first = 40 + new // 2 + 1  # seen by the rows from here on, where there are any
+    for frame in range(first, 40 + new):
+        put(c, c.v, frame, 0.0)
+    want = c.run().clone()
+    for frame in range(first, 40 + new):
+        put(c, c.v, frame, big if frame % 2 else -big)
+    got = c.run()
+    assert torch.equal(got[:first - 40], want[:first - 40])

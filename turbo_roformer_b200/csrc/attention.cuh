@@ -67,10 +67,13 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays <= 2^8
 // 2^x for a pair of fp32 values on the FMA pipe (no MUFU): x = j + f with j = round(x) (the 1.5 * 2^23
 // rounding constant), 2^f on [-1/2, 1/2] by a degree-3 polynomial fitted here for minimum relative error
 // (Chebyshev-node least squares with Lawson reweighting; max relative error 7.5e-5, below half an fp16
-// ulp), and j added to the exponent field. x is clamped at -126 so the exponent field never wraps; the
-// inputs here are <= 2^8 and results below 2^-24 flush to zero in the 16-bit P anyway.
+// ulp), and j added to the exponent field. x is clamped just above -127, where the exponent field is zero and the
+// polynomial is 1 + 2^-8.6, so that hidden scores (-inf) come out as 2^-134.6, which rounds to zero in both 16-bit
+// types (bf16 holds 2^-126: a clamp there would let hidden values of 1e38 through). Between the clamp and -126 results
+// are subnormal, off by less than 2^-126; the inputs here are <= 2^8. NaN is clamped too.
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  constexpr float kLeast = -126.99609375f;  // -127 + 2^-8
+  x = make_float2(fmaxf(x.x, kLeast), fmaxf(x.y, kLeast));
   const float2 round_c = make_float2(12582912.0f, 12582912.0f);
   const float2 t = __fadd2_rn(x, round_c);
   const float2 j = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));

@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(CtSmem<SHARED>::kThreads, 1)
         if (j == b && pending) finish();
       }
       if (!ok) break;
-      // a row that saw no key: ex2_poly2 makes 2^-126 of a hidden score, so its weight is set to zero here
+      // a row that saw no key: ex2_poly2 makes 2^-134.6 of a hidden score, so its weight is set to zero here
       if (m_run == -INFINITY) l_run = 0.f;
       *row_scale = l_run == 0.f ? 0.f : gate / l_run;
       dst_part = run.slot >= 0;
