@@ -243,7 +243,8 @@ int trc_add_rmsnorm(trc_handle* h, float* d_X, const float* d_Y, void* d_out, in
 int trc_qkv_rope_gemm(trc_handle* h, int layer, const void* d_xn, int batch, int T, void* d_Q, void* d_K, void* d_V,
                       float* d_G, void* stream);
 
-/* kernels.cpp:255-388 attention (mode 0 = time, 1 = freq): O = merge_heads(softmax(Q K^T) V * G). */
+/* kernels.cpp:255-388 attention (mode 0 = time, 1 = freq): O = merge_heads(softmax(Q K^T) V * G). A score of NaN or
+ * +inf makes its row NaN. */
 int trc_attention(trc_handle* h, int mode, const void* d_Q, const void* d_K, const void* d_V, const float* d_G,
                   void* d_O, int batch, int T, void* stream);
 

@@ -70,7 +70,7 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: P stays <= 2^8
 // ulp), and j added to the exponent field. x is clamped just above -127, where the exponent field is zero and the
 // polynomial is 1 + 2^-8.6, so that hidden scores (-inf) come out as 2^-134.6, which rounds to zero in both 16-bit
 // types (bf16 holds 2^-126: a clamp there would let hidden values of 1e38 through). Between the clamp and -126 results
-// are subnormal, off by less than 2^-126; the inputs here are <= 2^8. NaN is clamped too.
+// are subnormal, off by less than 2^-126; the inputs here are <= 2^8. NaN is clamped too: callers carry it in the maximum.
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   constexpr float kLeast = -126.99609375f;  // -127 + 2^-8
   x = make_float2(fmaxf(x.x, kLeast), fmaxf(x.y, kLeast));

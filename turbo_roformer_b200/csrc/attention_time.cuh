@@ -296,26 +296,29 @@ __global__ void __launch_bounds__(kTaThreads, 1)
           for (int i = 0; i < 64; ++i)
             if (i >= kmax) sc[i] = -INFINITY;
         }
+        // a score of NaN or +inf makes the row NaN, through its maximum: the polynomial would lose a NaN
         float mx4[4] = {sc[0], sc[1], sc[2], sc[3]};
 #pragma unroll
         for (int i = 4; i < 60; i += 8) {
-          mx4[0] = fmax3(mx4[0], sc[i], sc[i + 4]);
-          mx4[1] = fmax3(mx4[1], sc[i + 1], sc[i + 5]);
-          mx4[2] = fmax3(mx4[2], sc[i + 2], sc[i + 6]);
-          mx4[3] = fmax3(mx4[3], sc[i + 3], sc[i + 7]);
+          mx4[0] = fmax3_nan(mx4[0], sc[i], sc[i + 4]);
+          mx4[1] = fmax3_nan(mx4[1], sc[i + 1], sc[i + 5]);
+          mx4[2] = fmax3_nan(mx4[2], sc[i + 2], sc[i + 6]);
+          mx4[3] = fmax3_nan(mx4[3], sc[i + 3], sc[i + 7]);
         }
-        const float m_tile =
-            fmaxf(fmax3(mx4[0], mx4[1], sc[60]), fmax3(mx4[2], mx4[3], fmax3(sc[61], sc[62], sc[63]))) * kLog2e;
+        const float m_tile = fmax3_nan(fmax3_nan(mx4[0], mx4[1], sc[60]), fmax3_nan(mx4[2], mx4[3], sc[61]),
+                                       fmax3_nan(sc[62], sc[63], sc[63])) *
+                             kLog2e;
         bool rescale = false;
         float alpha = 1.0f;
         if (j == 0) {
-          m_run = m_tile;
+          m_run = m_tile < INFINITY ? m_tile : NAN;
         } else {
-          const bool need = m_tile > m_run + kRescaleThreshold;
+          const bool need = !(m_tile <= m_run + kRescaleThreshold);
           rescale = __any_sync(0xffffffffu, need);
           if (need) {
-            alpha = ex2_approx(m_run - m_tile);
-            m_run = m_tile;
+            const float m_next = m_tile < INFINITY ? m_tile : NAN;
+            alpha = ex2_approx(m_run - m_next);
+            m_run = m_next;
           }
         }
         const float2 scale2 = make_float2(kLog2e, kLog2e);
