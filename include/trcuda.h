@@ -163,7 +163,8 @@ int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t*
  * longer than cu[n_seqs] rows (a captured graph's capacity); the rows behind stay as they were.
  * Lengths, tables and slots live on the device and are not trusted: bad ones touch no memory outside the
  * buffers. They set *d_status (int32 on the device, may be NULL) or the plan's flags, and leave the outputs of
- * the sequences concerned undefined. */
+ * the sequences concerned undefined. For the attention, bad lengths are offsets that fall or leave the rows and, where
+ * there are new frames, totals below 0 or above table_stride * page. */
 #define TRC_CACHE_PLAN_MAX_SEQS 8192
 #define TRC_CACHE_MAX_SEQS 2048  /* sequences of one trc_cache_attention */
 #define TRC_CACHE_MAX_GROUP 64   /* query heads per cache head */

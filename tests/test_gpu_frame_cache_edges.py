@@ -87,3 +87,43 @@ def test_hidden_values_of_any_finite_size(cuda_device, dtype, big, new):
         put(c, c.v, frame, big if frame % 2 else -big)
     got = c.run()
     assert torch.equal(got[:first - 40], want[:first - 40])
+
+
+# ------------------------------------------------------------------------------------------------ lengths
+@pytest.mark.parametrize("new", [1, 40, 300])
+def test_lengths_that_do_not_fit_set_the_status(cuda_device, new):
+    """Totals outside the table and offsets outside the rows are reported; the other sequence's rows are right."""
+    c = Case("fp16", [new, 2], [600, 90], 2, 2, 16)
+    c.table = np.pad(c.table, ((0, 0), (0, 2)), constant_values=0)  # valid pages behind: nothing else to stumble on
+    want = c.run().clone()
+    for total in (601 + 16 * c.table.shape[1], 2**31 - 1, 2**30 + 1, -1, -2**31):
+        c.total, status = [total, 90], ints([0])
+        got = c.run(status=status)
+        assert status.item() != 0, total
+        assert torch.equal(got[new:], want[new:])
+    c.total = [600, 90]
+    good = c.cu.copy()
+    for cu in ([-1, new, new + 2], [0, new, new + 3], [0, new, new - 1], [0, new, 2**31 - 1], [0, -2**31, 2]):
+        c.cu, status = np.array(cu), ints([0])
+        c.run(status=status)
+        assert status.item() != 0, cu
+    c.cu, status = good, ints([0])
+    assert torch.equal(c.run(status=status), want) and status.item() == 0
+    # fewer frames cached than pushed, and a sequence without new frames, are no errors
+    c.total = [new // 2, 90]
+    c.run(status=status)
+    c.cu, c.total = np.array([0, 0, 2]), [-7, 90]
+    c.run(status=status)
+    assert status.item() == 0
+
+
+def test_a_full_table_reaches_the_status(cuda_device):
+    """A stream that outgrows its table: the plan's flag, and the status of the attention that follows."""
+    table, dt = ints([[3, -1]]), torch.float16
+    k = torch.randn(6, 1, 16, 64, device="cuda").to(dt)
+    plan = cache_plan(ints([16]), ints([20]), table, ints([4, 5, 2]), 16, 20)
+    assert plan.counts.tolist() == [2, 2] and plan.total.tolist() == [36]
+    status = ints([0])
+    cache_attention(torch.randn(20, 1, 64, device="cuda").to(dt), k, k.clone(), table, plan.cu, plan.total, 20, 36,
+                    status=status)
+    assert status.item() != 0

@@ -70,15 +70,23 @@ struct CacheSeq {
   int tok, n, total;  // first row, new frames, frames in the cache
 };
 
-__device__ __forceinline__ CacheSeq cache_seq(const CacheAttnArgs& a, int r) {
+// Sequence r, its lengths cut to the rows and the table. `bad` becomes true where they had to be: offsets that fall or
+// leave the rows, or, for a sequence with new frames, a total that is negative or more than the table holds.
+__device__ __forceinline__ CacheSeq cache_seq(const CacheAttnArgs& a, int r, bool& bad) {
+  const int from = a.cu[r], to = a.cu[r + 1], total = a.total[r];
+  const int room = (int)min((int64_t)a.table_stride << a.page_log2, (int64_t)1 << 30);
   CacheSeq s;
-  s.tok = min(max(a.cu[r], 0), a.n_tokens);
-  s.n = min(max(a.cu[r + 1], s.tok), a.n_tokens) - s.tok;
-  const int64_t room = min((int64_t)a.table_stride << a.page_log2, (int64_t)1 << 30);
-  s.total = (int)min((int64_t)max(a.total[r], 0), room);
+  s.tok = min(max(from, 0), a.n_tokens);
+  s.n = min(max(to, s.tok), a.n_tokens) - s.tok;
+  s.total = min(max(total, 0), room);
+  bad |= from < 0 || to < from || to > a.n_tokens || (to > from && s.total != total);
   const int64_t rows = (int64_t)s.n * a.group;
   if (rows <= a.rows_above || rows > a.rows_upto) s.n = 0;  // another launch's
   return s;
+}
+__device__ __forceinline__ CacheSeq cache_seq(const CacheAttnArgs& a, int r) {
+  bool bad = false;
+  return cache_seq(a, r, bad);
 }
 
 // Keys [lo, hi) that new frame i of a sequence sees.
@@ -151,16 +159,17 @@ __device__ __forceinline__ int64_t cache_share(const CacheAttnArgs& a, int64_t l
 // The line's scan, by all `threads` threads of the CTA: prefix[r] = places before sequence r, prefix[n_seqs] =
 // the line's length. Returns whether shares end inside items: not where the host rules it out, nor where a share
 // holds whole_from of the longest items (whole items are then at most 1 / whole_from uneven, nothing is joined).
-// `part` holds 32 int64 of scratch. Ends with a CTA barrier.
+// Block 0 reports lengths that do not fit. `part` holds 32 int64 of scratch. Ends with a CTA barrier.
 __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int threads, int ctas, int64_t* prefix,
                                            int64_t* part) {
   const int per = (a.n_seqs + threads - 1) / threads;
   const int r0 = min((int)threadIdx.x * per, a.n_seqs), r1 = min(r0 + per, a.n_seqs);
   int64_t sum = 0;
   int longest = 0;
+  bool bad = false;
   for (int r = r0; r < r1; ++r) {
     CacheItem it;
-    it.s = cache_seq(a, r);
+    it.s = cache_seq(a, r, bad);
     int64_t steps = 0;
     for (it.tile = 0; it.tile * tpt < it.s.n; ++it.tile) {
       it.set_tile(a, tpt);
@@ -186,7 +195,9 @@ __device__ __forceinline__ bool cache_scan(const CacheAttnArgs& a, int tpt, int 
   }
   for (int r = r0; r < r1; ++r) prefix[r] += before;
   if (threadIdx.x == 0) prefix[a.n_seqs] = length;
-  return __syncthreads_or(a.split && longest * (int64_t)a.whole_from > cache_share(a, length, ctas));
+  const bool divided = __syncthreads_or(a.split && longest * (int64_t)a.whole_from > cache_share(a, length, ctas));
+  if (bad && blockIdx.x == 0) record_error(a.status, kErrBadArgs);
+  return divided;
 }
 
 // The runs of steps that one worker works on, in order.

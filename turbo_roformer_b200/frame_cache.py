@@ -11,7 +11,8 @@ per stream takes three calls, all on the tensors' device and its current stream,
 Layouts are those of ``include/trcuda.h``: pools (pages, cache heads, page, 64), a frame's heads being all bands'
 heads; rows of all streams packed one behind the other; rows behind the last one are left as they were. Each call
 can be captured in a CUDA graph. ``status`` (an int32 tensor of one element, zeroed by the caller) receives a
-nonzero code when a kernel met a bad page or slot number; the plan's flags are in ``counts[1]``.
+nonzero code when a kernel met a bad page or slot number, or lengths that do not fit the rows or the table; the plan's
+flags are in ``counts[1]``.
 
 Tensors are checked (``ValueError``), results allocated and the library called in the extension module
 ``_cache_binding`` (``csrc/cache_binding.cpp``), because a push's kernels are shorter than these take in Python.
