@@ -178,7 +178,8 @@ int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t*
  * Sequences take the pages they lack, in order, from the front of d_free [n_free] into d_table (in place; other
  * entries are kept). Writes d_cu [n_seqs + 1], d_total [n_seqs] (cached + new), d_slots and d_positions
  * [max_rows] (frame number within the stream; rows behind the last get slot -1, position 0) and d_counts [2]:
- * pages taken from d_free, and the flags above (0 = none). */
+ * pages taken from d_free, and the flags above (0 = none). What is written overlaps nothing else (refused): a push's
+ * d_total is the next one's d_cached only as a copy. */
 int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, int page, const int32_t* d_free,
                    int n_free, int32_t* d_table, int table_stride, int max_rows, int32_t* d_cu, int32_t* d_total,
                    int32_t* d_slots, int32_t* d_positions, int32_t* d_counts, void* stream);

@@ -127,3 +127,21 @@ def test_a_full_table_reaches_the_status(cuda_device):
     cache_attention(torch.randn(20, 1, 64, device="cuda").to(dt), k, k.clone(), table, plan.cu, plan.total, 20, 36,
                     status=status)
     assert status.item() != 0
+
+
+# ------------------------------------------------------------------------------------------------ overlapping buffers
+def test_plan_refuses_buffers_that_overlap(cuda_device):
+    cached, new, table, free = ints([3, 4]), ints([2, 0]), ints([[0, -1], [1, -1]]), ints([5, 6])
+    p = cache_plan(cached, new, table, free, 16, 4)
+    for bad in (p._replace(total=cached), p._replace(total=new), p._replace(slots=p.positions),
+                p._replace(slots=table.view(-1)), p._replace(counts=free)):
+        with pytest.raises(Exception, match="overlap"):
+            cache_plan(cached, new, table, free, 16, 4, out=bad)
+    with pytest.raises(Exception, match="overlap"):
+        cache_plan(p.total, new, table, free, 16, 4, out=p)
+    with pytest.raises(Exception, match="overlap"):
+        cache_plan(cached, cached, table, table.view(-1)[2:], 16, 4)
+    cache_plan(cached, cached, table, free, 16, 4)  # inputs may be the same
+    one = ints(np.zeros(3 + 2 + 4 + 4 + 2))  # results side by side in one buffer
+    q = type(p)(*torch.split(one, [3, 2, 4, 4, 2]))
+    assert torch.equal(cache_plan(cached, new, table, free, 16, 4, out=q).positions, p.positions)

@@ -59,6 +59,24 @@ int page_log2_of(int page) {
   }
 }
 
+// Memory that a call reads or writes.
+struct Span {
+  const void* at;
+  int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.bytes > 0 && b.bytes > 0 && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+}
+// Whether one of the first `written` spans shares memory with another span.
+template <int N>
+bool overlap(const Span (&spans)[N], int written) {
+  for (int i = 0; i < written; ++i)
+    for (int k = i + 1; k < N; ++k)
+      if (overlap(spans[i], spans[k])) return true;
+  return false;
+}
+
 // ------------------------------------------------------------------------------------------------ plan
 // Every block repeats the scan over the sequences (two 64-bit sums per thread) and then takes its part of two
 // flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows, four at a time (one
@@ -500,6 +518,18 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
   if (lp < 0) return set_last_error(TRC_E_INVALID, "cache plan: page must be 16, 32, 64 or 128 frames");
   if (n_free < 0 || table_stride < 1 || max_rows < 0)
     return set_last_error(TRC_E_INVALID, "cache plan: bad sizes");
+  // every block reads all lengths while others already write
+  const trc::Span spans[] = {{d_table, 4ll * n_seqs * table_stride},
+                             {d_cu, 4ll * (n_seqs + 1)},
+                             {d_total, 4ll * n_seqs},
+                             {d_slots, 4ll * max_rows},
+                             {d_positions, 4ll * max_rows},
+                             {d_counts, 8},
+                             {d_cached, 4ll * n_seqs},
+                             {d_new, 4ll * n_seqs},
+                             {d_free, 4ll * n_free}};
+  if (trc::overlap(spans, 6))
+    return set_last_error(TRC_E_INVALID, "cache plan: what is written overlaps another argument");
   trc::PlanArgs a;
   a.cached = d_cached;
   a.fresh = d_new;

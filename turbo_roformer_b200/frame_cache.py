@@ -67,7 +67,8 @@ def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, fre
                max_rows: int, out: CachePlan | None = None) -> CachePlan:
     """Pages, slots and positions of a push: ``cached`` and ``new`` (sequences,) int32 frames each sequence has and
     gets. Sequences take the pages they lack from the front of ``free_pages`` into ``table`` (sequences, columns),
-    in place; ``max_rows`` is the capacity of the per-row outputs. ``out``: a plan to write into."""
+    in place; ``max_rows`` is the capacity of the per-row outputs. ``out``: a plan to write into; its ``total`` is not ``cached``
+    (kept lengths are advanced by ``cached += new`` after the push)."""
     r = (_binding or _load()).plan(cached, new, table, free_pages, page, max_rows, out)
     return r if r is out else CachePlan._make(r)
 
