@@ -191,7 +191,8 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
  * NULL: no rotation). d_q [n_rows][bands * heads][64], q_stride elements between frames; k and v go to
  * d_slots[row] of the pools (bands * kv_heads cache heads); d_gates [n_rows][bands * heads] fp32 = sigmoid
  * (NULL: none). Rows of slot < 0 are skipped; a slot behind the pool is not written and sets *d_status. Row
- * starts and d_freqs are 16-byte aligned; at most 1,048,560 rows, 4,096 bands and 4,096 heads per band. */
+ * starts and d_freqs are 16-byte aligned; at most 1,048,560 rows, 4,096 bands and 4,096 heads per band. What is written
+ * overlaps nothing else (refused), but with one band d_q may be d_qkv (q_stride = row_stride): q in its place. */
 int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64_t band_stride, int n_rows, int bands,
                      int heads, int kv_heads, const int32_t* d_positions, const int32_t* d_slots, const float* d_freqs,
                      int page, int n_pages, void* d_q, int64_t q_stride, void* d_k, void* d_v, float* d_gates,
@@ -210,7 +211,7 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
  * row NaN; one of -inf weighs nothing (a row of such scores only is zero). d_workspace is not used where
  * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are
  * finite; what the pages hold behind `total`, or wholly before every row's window, is not read into any result. d_out
- * does not overlap d_q. */
+ * and d_workspace overlap nothing else (refused); d_out may be other columns of the buffer that holds d_q. */
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
                         const int32_t* d_table, int table_stride, const int32_t* d_cu, const int32_t* d_total,
                         int n_seqs, int n_rows, int max_new, int max_total, int heads, int kv_heads, int page,

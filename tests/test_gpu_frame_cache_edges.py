@@ -145,3 +145,41 @@ def test_plan_refuses_buffers_that_overlap(cuda_device):
     one = ints(np.zeros(3 + 2 + 4 + 4 + 2))  # results side by side in one buffer
     q = type(p)(*torch.split(one, [3, 2, 4, 4, 2]))
     assert torch.equal(cache_plan(cached, new, table, free, 16, 4, out=q).positions, p.positions)
+
+
+def test_append_refuses_buffers_that_overlap(cuda_device):
+    dt, i = torch.float16, ints([0, 1, 2])
+    qkv = torch.randn(3, 1, 256, device="cuda").to(dt)
+    k = torch.zeros(2, 1, 16, 64, dtype=dt, device="cuda")
+    v = torch.zeros_like(k)
+    call = lambda **kw: cache_append(**{**dict(qkv=qkv, positions=i, slots=i, k_pages=k, v_pages=v, heads=2, kv_heads=1,  # noqa: E731
+                                               freqs=None), **kw})
+    for bad in (dict(v_pages=k), dict(q=qkv[:, 0, 64:192].view(3, 2, 64)), dict(q=k.view(-1)[:384].view(3, 2, 64)),
+                dict(q=qkv.view(-1)[:384].view(3, 2, 64))):
+        with pytest.raises(Exception, match="overlap"):
+            call(**bad)
+    # q of a row over the row's own q, and beside it
+    freqs = torch.from_numpy(FREQS).cuda()
+    want = call(freqs=freqs)[0].clone()
+    kept_k, kept_v = k.clone(), v.clone()
+    wide = torch.zeros(3, 1, 384, dtype=dt, device="cuda")
+    wide[..., :256] = qkv
+    call(qkv=wide[..., :256], q=wide[:, 0, 256:].view(3, 2, 64), freqs=freqs)
+    assert torch.equal(wide[:, 0, 256:].reshape(3, 2, 64), want) and torch.equal(wide[..., :256], qkv)
+    call(q=qkv[:, 0, :128].view(3, 2, 64), freqs=freqs)
+    assert torch.equal(qkv[:, 0, :128].reshape(3, 2, 64), want)
+    assert torch.equal(k, kept_k) and torch.equal(v, kept_v) and torch.equal(wide[..., 128:256], qkv[..., 128:])
+
+
+def test_attention_refuses_buffers_that_overlap(cuda_device):
+    c = Case("fp16", [3], [20], 2, 2, 16)
+    wide = torch.zeros(3, 6, 64, dtype=c.dtype, device="cuda")
+    wide[:, 1:3] = c.q
+    want = c.run().clone()
+    flat = wide.view(-1)
+    c.q = wide[:, 1:3]
+    for bad in (c.q, wide[:, 2:4], wide[:, 0:2], flat[64:64 + 384].view(3, 2, 64), c.k.view(-1)[:384].view(3, 2, 64),
+                c.v.view(-1)[-384:].view(3, 2, 64)):
+        with pytest.raises(Exception, match="overlap"):
+            c.run(bad)
+    assert torch.equal(c.run(wide[:, 3:5]), want)  # beside q in the same rows

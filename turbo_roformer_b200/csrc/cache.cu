@@ -77,6 +77,25 @@ bool overlap(const Span (&spans)[N], int written) {
   return false;
 }
 
+// Rows `width` bytes long, `stride` bytes apart.
+struct Rows {
+  const void* at;
+  int64_t stride, width;
+  Span span(int64_t n) const {
+    const int64_t reach = (n - 1) * stride;  // negative: the first row lies last
+    return {static_cast<const char*>(at) + (reach < 0 ? reach : 0), (reach < 0 ? -reach : reach) + width};
+  }
+};
+// Whether any of n rows of a and n of b share memory. Rows of one stride may lie between each other's (columns of a
+// wider buffer); of different strides they count as overlapping where their spans do. a.stride >= a.width.
+bool overlap(const Rows& a, const Rows& b, int64_t n) {
+  if (!overlap(a.span(n), b.span(n))) return false;
+  if (n == 1 || a.stride != b.stride) return true;
+  const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(b.at) - reinterpret_cast<uintptr_t>(a.at));
+  const int64_t d = ((apart % a.stride) + a.stride) % a.stride;  // where in a row of a, or behind it, rows of b begin
+  return d < a.width || d + b.width > a.stride;
+}
+
 // ------------------------------------------------------------------------------------------------ plan
 // Every block repeats the scan over the sequences (two 64-bit sums per thread) and then takes its part of two
 // flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows, four at a time (one
@@ -585,6 +604,25 @@ int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64
     return set_last_error(TRC_E_INVALID, "cache append: rows (and d_freqs) must start on 16-byte boundaries");
   if ((bands > 1 && band_stride < width) || (n_rows > 1 && q_stride < (int64_t)bands * heads * 64))
     return set_last_error(TRC_E_INVALID, "cache append: strides shorter than the rows");
+  if (n_rows > 1 << 20 || (n_rows + trc::kAppendFrames - 1) / trc::kAppendFrames > 65535)  // the grid's second axis
+    return set_last_error(TRC_E_INVALID, "cache append: more than 1,048,560 rows");
+  // threads write what others have yet to read; only a row's q may take the place of the q it is made from
+  const int64_t qkv_width = 2 * ((bands - 1) * band_stride + width), page_bytes = 128ll * bands * kv_heads * page;
+  const int64_t pool = n_pages > (1ll << 62) / page_bytes ? 1ll << 62 : n_pages * page_bytes;
+  const trc::Rows from = {d_qkv, 2 * row_stride, qkv_width}, to = {d_q, 2 * q_stride, 128ll * bands * heads};
+  const trc::Span spans[] = {{d_k, pool},
+                             {d_v, pool},
+                             {d_gates, d_gates ? 4ll * n_rows * bands * heads : 0},
+                             to.span(n_rows),
+                             from.span(n_rows),
+                             {d_positions, 4ll * n_rows},
+                             {d_slots, 4ll * n_rows},
+                             {d_freqs, d_freqs ? 128 : 0}};
+  const bool in_place =
+      d_q == d_qkv && bands == 1 && (n_rows == 1 || (q_stride == row_stride && row_stride >= width));
+  if (trc::overlap(spans, 3) || trc::overlap(to.span(n_rows), spans[5]) || trc::overlap(to.span(n_rows), spans[6]) ||
+      trc::overlap(to.span(n_rows), spans[7]) || (!in_place && trc::overlap(to, from, n_rows)))
+    return set_last_error(TRC_E_INVALID, "cache append: what is written overlaps another argument");
   trc::AppendArgs a;
   a.qkv = d_qkv;
   a.tok_stride = row_stride;
@@ -604,8 +642,6 @@ int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64
   a.kv_heads = kv_heads;
   a.page_log2 = lp;
   a.n_slots = (int64_t)n_pages << lp;
-  if (n_rows > 1 << 20 || (n_rows + trc::kAppendFrames - 1) / trc::kAppendFrames > 65535)  // the grid's second axis
-    return set_last_error(TRC_E_INVALID, "cache append: more than 1,048,560 rows");
   const int sms = trc::sm_count();
   if (!sms) return set_last_error(TRC_E_CUDA, "cache append: no current CUDA device");
   // the most frames per block that leave eight blocks per SM
@@ -657,6 +693,19 @@ int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const 
     return set_last_error(TRC_E_INVALID, "cache attention: rows must start on 16-byte boundaries");
   if (n_rows > 1 && (q_stride < (int64_t)heads * 64 || out_stride < (int64_t)heads * 64))
     return set_last_error(TRC_E_INVALID, "cache attention: strides shorter than the rows");
+  const trc::Rows to = {d_out, 2 * out_stride, 128ll * heads};
+  const int64_t pool = 128ll * n_pages * kv_heads * page;
+  const trc::Span spans[] = {to.span(n_rows),
+                             {d_workspace, d_workspace ? workspace_bytes : 0},
+                             {d_k, pool},
+                             {d_v, pool},
+                             {d_table, 4ll * n_seqs * table_stride},
+                             {d_cu, 4ll * (n_seqs + 1)},
+                             {d_total, 4ll * n_seqs},
+                             {d_gates, d_gates ? 4ll * n_rows * heads : 0}};
+  const trc::Rows from = {d_q, 2 * q_stride, 128ll * heads};
+  if (trc::overlap(spans, 2) || trc::overlap(spans[1], from.span(n_rows)) || trc::overlap(to, from, n_rows))
+    return set_last_error(TRC_E_INVALID, "cache attention: what is written overlaps another argument");
   const int sms = trc::sm_count();
   if (!sms) return set_last_error(TRC_E_CUDA, "cache attention: no current CUDA device");
   trc::CacheAttnArgs a;

@@ -84,7 +84,7 @@ def cache_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     frequencies (the checkpoint's ``rotary_embed.freqs``), None for no rotation. Returns q (rows, bands * heads,
     64) and the sigmoid gates (rows, bands * heads) fp32, or None; ``q`` and ``gates`` may be tensors to write into
     (``gates=True``: a new one). Rows whose slot is -1 are skipped: where q and gates are new, their values there
-    are undefined."""
+    are undefined. What is written overlaps no other argument; only with one band may ``q`` be the q of ``qkv`` itself."""
     return (_binding or _load()).append(qkv, positions, slots, k_pages, v_pages, heads, kv_heads, freqs, q, gates,
                                         status)
 
@@ -97,7 +97,7 @@ def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     against frames 0 .. total[i] - 1 of each sequence, the new ones being the last. ``causal``: a frame sees none
     after it; ``window`` > 0: only that many up to itself. ``gates`` (rows, heads) fp32 scale the result, which is
     zero for a frame that sees nothing. ``max_new`` / ``max_total``: the longest new part and total as far as the
-    host knows; they choose the kernel variant only. ``out``: where to write (not over ``q``); otherwise a new
+    host knows; they choose the kernel variant only. ``out``: where to write (not over another argument); otherwise a new
     tensor, undefined in rows behind the last sequence's."""
     return (_binding or _load()).attention(q, k_pages, v_pages, table, cu, total, max_new, max_total, causal, window,
                                            scale, gates, out, status)
