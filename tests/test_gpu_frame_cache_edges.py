@@ -129,6 +129,34 @@ def test_a_full_table_reaches_the_status(cuda_device):
     assert status.item() != 0
 
 
+def test_plan_of_absurd_lengths_ends_soon(cuda_device):
+    """Lengths of up to 2^30 frames in every sequence name 2^39 pages: the work stays that of the table and the rows."""
+    n, page, rows, free = 8192, 16, 50, [11, 12, 13]
+    cached, new = np.full(n, 0), np.full(n, 2**30)
+    cached[0], new[0] = 5, 30  # two pages of its own first
+    table = ints(np.full((n, 3), 77))
+    args = ints(cached), ints(new)
+    p = cache_plan(*args, table, ints(free), page, rows)
+    torch.cuda.synchronize()
+    t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    t0.record()
+    p = cache_plan(*args, table, ints(free), page, rows, out=p)
+    t1.record()
+    torch.cuda.synchronize()
+    want = np.full((n, 3), -1)
+    want[0] = 77, 11, 12
+    want[1, 0] = 13
+    assert np.array_equal(table.cpu().numpy(), want)
+    assert p.counts.tolist() == [3, CO.NO_PAGES | CO.TABLE_FULL | CO.ROWS_FULL]
+    assert p.cu[:3].tolist() == [0, 30, 30 + 2**30] and p.cu[-1].item() == 2**31 - 1
+    slots = [77 * 16 + x for x in range(5, 16)] + [11 * 16 + x for x in range(16)] + [12 * 16 + x for x in range(3)]
+    assert p.slots.tolist() == slots + [13 * 16 + x for x in range(16)] + [-1] * 4
+    assert p.positions.tolist() == [*range(5, 35), *range(20)]
+    # 8,192 sequences in 32 warps are some thousand steps of well under a microsecond; 2^31 pages in 1,024 threads would
+    # be two million steps each
+    assert t0.elapsed_time(t1) < 50, t0.elapsed_time(t1)
+
+
 # ------------------------------------------------------------------------------------------------ overlapping buffers
 def test_plan_refuses_buffers_that_overlap(cuda_device):
     cached, new, table, free = ints([3, 4]), ints([2, 0]), ints([[0, -1], [1, -1]]), ints([5, 6])

@@ -129,6 +129,15 @@ __device__ __forceinline__ int last_upto(const int32_t* v, int n, int at) {
   return x;
 }
 
+// A sequence's lengths, 0 and 0 (and true) where they are bad.
+__device__ __forceinline__ bool plan_lengths(const PlanArgs& a, int r, int& c, int& n) {
+  c = a.cached[r];
+  n = a.fresh[r];
+  const bool bad = c < 0 || n < 0 || (int64_t)c + n > (1 << 30);
+  if (bad) c = n = 0;
+  return bad;
+}
+
 __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_constant__ PlanArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* cu = plan_smem;                   // [n_seqs + 1] rows before each sequence
@@ -142,11 +151,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
   // the new lengths pass through cu
   int bad = 0;
   for (int r = threadIdx.x; r < a.n_seqs; r += kPlanThreads) {
-    int c = a.cached[r], n = a.fresh[r];
-    if (c < 0 || n < 0 || (int64_t)c + n > (1 << 30)) {
-      bad |= TRC_CACHE_BAD_LENGTH;
-      c = n = 0;
-    }
+    int c, n;
+    if (plan_lengths(a, r, c, n)) bad |= TRC_CACHE_BAD_LENGTH;
     cached[r] = c;
     cu[r] = n;
     if (pages_of(c + n, a.page_log2) > a.table_stride) bad |= TRC_CACHE_TABLE_FULL;
@@ -216,16 +222,28 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
   for (int r = first; r <= a.n_seqs; r += stride) {
     a.cu[r] = cu[r];
     if (r < a.n_seqs) {
-      const int c = a.cached[r], n = a.fresh[r];  // as above: bad lengths count as none
-      a.total[r] = c < 0 || n < 0 || (int64_t)c + n > (1 << 30) ? 0 : c + n;
+      int c, n;
+      plan_lengths(a, r, c, n);
+      a.total[r] = c + n;
     }
   }
   // fresh pages into the table
-  for (int64_t e = first; e < live_pages; e += stride) {
+  const int64_t given = min(live_pages, a.n_free);
+  for (int64_t e = first; e < given; e += stride) {
     const int r = last_upto(base, a.n_seqs, (int)e);
     const int64_t column = (int64_t)pages_of(cached[r], a.page_log2) + (e - base[r]);
-    if (column < a.table_stride)
-      a.table[(int64_t)r * a.table_stride + column] = e < a.n_free ? a.free_pages[e] : -1;
+    if (column < a.table_stride) a.table[(int64_t)r * a.table_stride + column] = a.free_pages[e];
+  }
+  // entries that the free list no longer serves, a warp per sequence: the work is the table's, whatever the lengths are
+  if (live_pages > a.n_free) {
+    for (int r = first >> 5; r < a.n_seqs; r += stride >> 5) {
+      int c, n;
+      plan_lengths(a, r, c, n);
+      const int need = min(pages_of(c + n, a.page_log2), a.table_stride);
+      for (int64_t column = (int64_t)pages_of(c, a.page_log2) + max(a.n_free - base[r], 0) + lane; column < need;
+           column += 32)
+        a.table[(int64_t)r * a.table_stride + column] = -1;
+    }
   }
   // rows: position and slot, four to a thread
   auto store4 = [&](int32_t* to, int64_t row0, const int(&v)[4]) {
