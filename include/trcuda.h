@@ -166,7 +166,7 @@ int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t*
  * the sequences concerned undefined. For the attention, bad lengths are offsets that fall or leave the rows and, where
  * there are new frames, totals below 0 or above table_stride * page. */
 #define TRC_CACHE_PLAN_MAX_SEQS 8192
-#define TRC_CACHE_MAX_SEQS 2048  /* sequences of one trc_cache_attention */
+#define TRC_CACHE_MAX_SEQS 2048  /* sequences of one trc_cache_attention; a longer plan takes several, over slices */
 #define TRC_CACHE_MAX_GROUP 64   /* query heads per cache head */
 #define TRC_CACHE_MAX_WHOLE 512  /* up to this max_total, trc_cache_attention uses no workspace */
 #define TRC_CACHE_NO_PAGES 1     /* plan flags: the free list ran out (missing table entries and slots are -1) */

@@ -15,6 +15,46 @@ from .test_gpu_frame_cache import FREQS, Case, f64, ints, test_append_matches_or
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------------------------------------ append
+# Frames of a block: the most of 16, 8, 4, 2, 1 that leave eight blocks per SM (1,184 on 148 SMs). A thread then takes
+# every 32 / frames-th head row, four in flight: 8, 16, 32, 64 or 128 head rows at a time.
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("frames,rows,bands,heads,kv,page,gates,rope", [
+    (16, 18961, 1, 11, 1, 16, False, True), (16, 333, 62, 11, 1, 64, True, True), (16, 329, 62, 8, 8, 128, True, True),
+    (8, 161, 62, 18, 2, 32, True, True), (8, 9601, 1, 7, 7, 64, True, False), (4, 83, 62, 33, 3, 16, True, True),
+    (4, 5003, 1, 40, 8, 128, False, True), (2, 41, 60, 65, 5, 32, True, True), (1, 3, 2, 130, 10, 16, True, True)])
+def test_append_frames_of_a_block(cuda_device, dtype, frames, rows, bands, heads, kv, page, gates, rope):
+    """Every number of frames to a block, last blocks that are not full, rows without a slot beside live ones, and head
+    rows that take several passes with a ragged end."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    most = [f for f in (16, 8, 4, 2) if -(-rows // f) * bands >= 8 * sms]
+    assert sms != 148 or (most or [1])[0] == frames
+    assert rows % frames or frames == 1
+    check_append(cuda_device, dtype, rows, bands, heads, kv, page, 123456, gates, rope)
+
+
+def test_append_bad_slots_beside_good_ones(cuda_device):
+    """Blocks of 16 frames in which some slots lie behind the pool: those rows' k and v go nowhere, all others arrive."""
+    rows, bands, heads, kv, page, dt = 333, 62, 3, 1, 16, torch.float16
+    r = np.random.default_rng(8)
+    n_pages = -(-rows // page)
+    slots = r.permutation(n_pages * page)[:rows]
+    bad = r.random(rows) < 0.1
+    slots[bad] += n_pages * page
+    qkv = torch.randn(rows, bands, (heads + 2 * kv) * 64, device="cuda").to(dt)
+    k = torch.full((n_pages, bands * kv, page, 64), 7.0, dtype=dt, device="cuda")
+    v, status = torch.full_like(k, 8.0), ints([0])
+    q, _ = cache_append(qkv, ints(np.arange(rows)), ints(slots), k, v, heads, kv, freqs=None, status=status)
+    assert status.item() != 0
+    assert torch.equal(q, qkv[:, :, :heads * 64].reshape(rows, bands * heads, 64))
+    want_k, want_v = torch.full_like(k, 7.0), torch.full_like(v, 8.0)
+    good = torch.from_numpy(slots[~bad]).cuda()
+    rest = qkv[torch.from_numpy(~bad).cuda()]
+    want_k[good // page, :, good % page] = rest[:, :, heads * 64:(heads + kv) * 64]
+    want_v[good // page, :, good % page] = rest[:, :, (heads + kv) * 64:]
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
 # ------------------------------------------------------------------------------------------------ not finite
 VARIANTS = [1, 20, 60, 140, 400]  # new frames of one query head: every kernel form
 
@@ -155,6 +195,26 @@ def test_plan_of_absurd_lengths_ends_soon(cuda_device):
     # 8,192 sequences in 32 warps are some thousand steps of well under a microsecond; 2^31 pages in 1,024 threads would
     # be two million steps each
     assert t0.elapsed_time(t1) < 50, t0.elapsed_time(t1)
+
+
+# ------------------------------------------------------------------------------------------------ many sequences
+def test_one_plan_for_several_attention_calls(cuda_device):
+    """A plan of more sequences than one attention call takes: calls over slices of its table, offsets and totals."""
+    r, page, n = np.random.default_rng(4), 16, 3000
+    new, total = r.integers(0, 3, n), r.integers(3, 40, n)
+    c = Case("bf16", new.tolist(), total.tolist(), 2, 1, page, pad=3)
+    table, cu, totals = ints(c.table), ints(c.cu), ints(c.total)
+    out, status = torch.full_like(c.q, 3.0), ints([0])
+    with pytest.raises(Exception, match="TRC_CACHE_MAX_SEQS"):
+        cache_attention(c.q, c.k, c.v, table, cu, totals, 2, 40)
+    for a, b in ((0, 2048), (2048, n)):
+        cache_attention(c.q, c.k, c.v, table[a:b], cu[a:b + 1], totals[a:b], 2, 40, out=out, status=status)
+    assert status.item() == 0 and (out[int(c.cu[-1]):] == 3.0).all()
+    for a in (0, 1500, 2040, 2900):  # the same rows from a call of their own
+        b = min(a + 100, n)
+        alone = cache_attention(c.q, c.k, c.v, table[a:b], cu[a:b + 1], totals[a:b], 2, 40)
+        x, y = int(c.cu[a]), int(c.cu[b])
+        assert torch.equal(alone[x:y], out[x:y])
 
 
 # ------------------------------------------------------------------------------------------------ overlapping buffers

@@ -97,7 +97,8 @@ def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     against frames 0 .. total[i] - 1 of each sequence, the new ones being the last. ``causal``: a frame sees none
     after it; ``window`` > 0: only that many up to itself. ``gates`` (rows, heads) fp32 scale the result, which is
     zero for a frame that sees nothing. ``max_new`` / ``max_total``: the longest new part and total as far as the
-    host knows; they choose the kernel variant only. ``out``: where to write (not over another argument); otherwise a new
+    host knows; they choose the kernel variant only. At most 2,048 sequences: of a longer plan, calls take slices
+    ``table[a:b]``, ``cu[a:b + 1]``, ``total[a:b]`` with the same ``q`` and ``out``. ``out``: where to write (not over another argument); otherwise a new
     tensor, undefined in rows behind the last sequence's."""
     return (_binding or _load()).attention(q, k_pages, v_pages, table, cu, total, max_new, max_total, causal, window,
                                            scale, gates, out, status)
