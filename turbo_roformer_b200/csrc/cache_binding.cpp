@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -65,6 +66,18 @@ struct Args {
   }
 };
 constexpr int64_t kInt = INT32_MAX;
+
+// The operators have no backward pass: a result without history in place of a gradient would be silent.
+const at::Tensor& plain(const at::Tensor& t, const char* name) {
+  need(!(c10::GradMode::is_enabled() && t.requires_grad()), name,
+       " requires grad, and the frame cache has no backward pass: call it under torch.no_grad()");
+  return t;
+}
+
+// Tells autograd that a tensor has new contents.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 const int32_t* ints(const at::Tensor& t, int device, int64_t ndim, const char* name) {
   need(t.scalar_type() == at::kInt && t.is_cuda() && t.get_device() == device && t.dim() == ndim && t.is_contiguous(), name,
@@ -147,7 +160,7 @@ PyObject* plan(const Args& a) {
   const at::Tensor& fresh = a.tensor(1, "new");
   const int32_t* n_new = ints(fresh, device, 1, "new");
   const at::Tensor& table = a.tensor(2, "table");
-  const int32_t* t = ints(table, device, 2, "table");
+  ints(table, device, 2, "table");
   const at::Tensor& free_pages = a.tensor(3, "free_pages");
   const int32_t* f = ints(free_pages, device, 1, "free_pages");
   const int64_t n = cached.size(0), columns = table.size(1);
@@ -168,7 +181,8 @@ PyObject* plan(const Args& a) {
       PyObject* o = PyTuple_GET_ITEM(a.v[6], i);
       need(THPVariable_Check(o), names[i], " must be a tensor");
       out[i] = THPVariable_Unpack(o);
-      p[i] = const_cast<int32_t*>(ints(out[i], device, 1, names[i]));
+      ints(out[i], device, 1, names[i]);
+      p[i] = out[i].data_ptr<int32_t>();
       need(out[i].size(0) == sizes[i], names[i], " has the wrong number of elements");
     }
   } else {
@@ -186,23 +200,27 @@ PyObject* plan(const Args& a) {
       p[i] = out[i].data_ptr<int32_t>();
     }
   }
-  const int rc = g_plan(c, n_new, (int)n, (int)page, f, (int)free_pages.size(0), const_cast<int32_t*>(t), (int)columns,
-                        (int)rows, p[0], p[1], p[2], p[3], p[4], on.stream);
+  const int rc = g_plan(c, n_new, (int)n, (int)page, f, (int)free_pages.size(0), table.data_ptr<int32_t>(),
+                        (int)columns, (int)rows, p[0], p[1], p[2], p[3], p[4], on.stream);
   if (rc) throw Failed{rc};
-  if (given) return same(a.v[6]);
+  written(table);
+  if (given) {
+    for (const at::Tensor& o : out) written(o);
+    return same(a.v[6]);
+  }
   return steal_tuple({wrap(out[0]), wrap(out[1]), wrap(out[2]), wrap(out[3]), wrap(out[4])});
 }
 
 // append(qkv, positions, slots, k, v, heads, kv_heads, freqs | None, q | None, gates | True | None, status | None)
 // -> (q, gates | None)
 PyObject* append(const Args& a) {
-  const at::Tensor& qkv = a.tensor(0, "qkv");
+  const at::Tensor& qkv = plain(a.tensor(0, "qkv"), "qkv");
   const int prec = precision_of(qkv);
   need(qkv.is_cuda() && qkv.dim() == 3 && prec >= 0, "qkv must be a (rows, bands, width) fp16 or bf16 CUDA tensor");
   const int device = qkv.get_device();
   const int64_t rows = qkv.size(0), bands = qkv.size(1), width = qkv.size(2);
-  const at::Tensor& k = a.tensor(3, "k_pages");
-  const at::Tensor& v = a.tensor(4, "v_pages");
+  const at::Tensor& k = plain(a.tensor(3, "k_pages"), "k_pages");
+  const at::Tensor& v = plain(a.tensor(4, "v_pages"), "v_pages");
   const int64_t heads = a.integer(5, "heads", 1, 4096), kv = a.integer(6, "kv_heads", 1, 4096);
   need(heads % kv == 0, "kv_heads must divide heads");
   const Pools pool = pools_of(k, v, qkv);
@@ -218,7 +236,7 @@ PyObject* append(const Args& a) {
   need(rows <= kInt, "too many rows");
   const float* fr = nullptr;
   if (!a.none(7)) {
-    const at::Tensor& freqs = a.tensor(7, "freqs");
+    const at::Tensor& freqs = plain(a.tensor(7, "freqs"), "freqs");
     need(freqs.scalar_type() == at::kFloat && freqs.is_cuda() && freqs.get_device() == device && freqs.dim() == 1 &&
              freqs.size(0) == kDim / 2 && freqs.is_contiguous(),
          "freqs must be 32 float32 on the first tensor's device");
@@ -227,12 +245,12 @@ PyObject* append(const Args& a) {
   int* status = status_of(a, 10, device);
   OnDevice on(device);
   const bool new_q = a.none(8);
-  const at::Tensor q = new_q ? at::empty({rows, bands * heads, kDim}, qkv.options()) : a.tensor(8, "q");
+  const at::Tensor q = new_q ? at::empty({rows, bands * heads, kDim}, qkv.options()) : plain(a.tensor(8, "q"), "q");
   const int64_t q_stride = row_stride(q, rows, bands * heads, qkv, "q");
   at::Tensor gates;
   float* g = nullptr;
   if (wanted) {
-    gates = new_gates ? at::empty({rows, bands * heads}, qkv.options().dtype(at::kFloat)) : a.tensor(9, "gates");
+    gates = new_gates ? at::empty({rows, bands * heads}, qkv.options().dtype(at::kFloat)) : plain(a.tensor(9, "gates"), "gates");
     g = gates_of(gates, rows, bands * heads, device);
   }
   if (rows) {
@@ -241,6 +259,10 @@ PyObject* append(const Args& a) {
                             (int)rows, (int)bands, (int)heads, (int)kv, pos, slot, fr, (int)pool.page, (int)pool.pages,
                             q.data_ptr(), q_stride, k.data_ptr(), v.data_ptr(), g, status, on.stream);
     if (rc) throw Failed{rc};
+    written(k);
+    written(v);
+    if (!new_q) written(q);
+    if (wanted && !new_gates) written(gates);
   }
   return steal_tuple({new_q ? wrap(q) : same(a.v[8]),
                       !wanted     ? same(Py_None)
@@ -251,13 +273,13 @@ PyObject* append(const Args& a) {
 // attention(q, k, v, table, cu, total, max_new, max_total, causal, window, scale, gates | None, out | None,
 // status | None) -> out
 PyObject* attention(const Args& a) {
-  const at::Tensor& q = a.tensor(0, "q");
+  const at::Tensor& q = plain(a.tensor(0, "q"), "q");
   const int prec = precision_of(q);
   need(q.is_cuda() && q.dim() == 3 && prec >= 0, "q must be a (rows, heads, 64) fp16 or bf16 CUDA tensor");
   const int device = q.get_device();
   const int64_t rows = q.size(0), heads = q.size(1);
-  const at::Tensor& k = a.tensor(1, "k_pages");
-  const at::Tensor& v = a.tensor(2, "v_pages");
+  const at::Tensor& k = plain(a.tensor(1, "k_pages"), "k_pages");
+  const at::Tensor& v = plain(a.tensor(2, "v_pages"), "v_pages");
   const Pools pool = pools_of(k, v, q);
   need(q.size(2) == kDim && heads >= 1 && heads <= kInt && pool.heads >= 1 && heads % pool.heads == 0,
        "q must have 64 elements per head, and the cache heads must divide its heads");
@@ -277,11 +299,11 @@ PyObject* attention(const Args& a) {
   const double scale = PyFloat_AsDouble(a.v[10]);
   if (scale == -1.0 && PyErr_Occurred()) throw python_error();
   const int64_t q_stride = row_stride(q, rows, heads, q, "q");
-  const float* g = a.none(11) ? nullptr : gates_of(a.tensor(11, "gates"), rows, heads, device);
+  const float* g = a.none(11) ? nullptr : gates_of(plain(a.tensor(11, "gates"), "gates"), rows, heads, device);
   int* status = status_of(a, 13, device);
   OnDevice on(device);
   const bool new_out = a.none(12);
-  const at::Tensor out = new_out ? at::empty({rows, heads, kDim}, q.options()) : a.tensor(12, "out");
+  const at::Tensor out = new_out ? at::empty({rows, heads, kDim}, q.options()) : plain(a.tensor(12, "out"), "out");
   const int64_t out_stride = row_stride(out, rows, heads, q, "out");
   if (rows) {
     at::Tensor held;  // of the current stream's pool: free for later work on it
@@ -296,6 +318,7 @@ PyObject* attention(const Args& a) {
                                (int)pool.heads, (int)pool.page, (int)pool.pages, causal, (int)window, (float)scale, g,
                                out.data_ptr(), out_stride, bytes ? held.data_ptr() : nullptr, bytes, status, on.stream);
     if (rc) throw Failed{rc};
+    if (!new_out) written(out);
   }
   return new_out ? wrap(out) : same(a.v[12]);
 }

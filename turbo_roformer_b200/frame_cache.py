@@ -14,6 +14,7 @@ can be captured in a CUDA graph. ``status`` (an int32 tensor of one element, zer
 nonzero code when a kernel met a bad page or slot number, or lengths that do not fit the rows or the table; the plan's
 flags are in ``counts[1]``.
 
+There is no backward pass: a tensor that requires grad is refused unless gradients are off (``torch.no_grad``).
 Tensors are checked (``ValueError``), results allocated and the library called in the extension module
 ``_cache_binding`` (``csrc/cache_binding.cpp``), because a push's kernels are shorter than these take in Python.
 """
