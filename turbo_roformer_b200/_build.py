@@ -11,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -40,6 +41,23 @@ def _source_hash() -> str:
     return h.hexdigest()[:16]
 
 
+def _compile(cmd: list[str], path: str, digest: str) -> str:
+    """Run a compiler whose output is to be ``path``, and note the sources it was made from. The output gets a name of
+    its own until it is whole, so that processes and threads that build at once do not write into each other's."""
+    tmp = f"{path}.{os.getpid()}.{threading.get_ident()}.tmp"
+    try:
+        res = subprocess.run([*cmd, "-o", tmp], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        os.replace(tmp, path)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+    with open(path + ".hash", "w") as f:
+        f.write(digest + "\n")
+    return path
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile the CUDA sources into ``turbo_roformer_b200/libtrcuda.so`` (skipped when up to date)."""
     stamp = LIB_PATH + ".hash"
@@ -59,19 +77,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         "-shared",
         "-I",
         INCLUDE,
-        "-o",
-        LIB_PATH + ".tmp",
         *(os.path.join(CSRC, s) for s in SOURCES),
     ]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    os.replace(LIB_PATH + ".tmp", LIB_PATH)
-    with open(stamp, "w") as f:
-        f.write(digest + "\n")
-    return LIB_PATH
+    return _compile(cmd, LIB_PATH, digest)
 
 
 BINDING_SOURCE = os.path.join(CSRC, "cache_binding.cpp")
@@ -104,8 +114,6 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
         *(f"-I{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"), cuda,
                              sysconfig.get_paths()["include"])),
         BINDING_SOURCE,
-        "-o",
-        BINDING_PATH + ".tmp",
         f"-L{lib}",
         "-ltorch_python",
         "-ltorch_cpu",
@@ -115,13 +123,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     ]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    os.replace(BINDING_PATH + ".tmp", BINDING_PATH)
-    with open(stamp, "w") as f:
-        f.write(digest + "\n")
-    return BINDING_PATH
+    return _compile(cmd, BINDING_PATH, digest)
 
 
 if __name__ == "__main__":
