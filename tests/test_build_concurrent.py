@@ -53,3 +53,31 @@ def test_failed_build_leaves_nothing(monkeypatch, tmp_path, build, path):
     with pytest.raises(RuntimeError, match="no such thing"):
         getattr(_build, build)(force=True)
     assert os.listdir(tmp_path) == []
+
+
+def test_binding_follows_the_header(monkeypatch, tmp_path):
+    """The binding takes the C ABI's signatures and limits from the header: a changed header means a new binding."""
+    include = tmp_path / "include"
+    include.mkdir()
+    with open(os.path.join(_build.INCLUDE, "trcuda.h")) as f:
+        text = f.read()
+    (include / "trcuda.h").write_text(text)
+    monkeypatch.setattr(_build, "BINDING_PATH", str(tmp_path / "lib.so"))
+    monkeypatch.setattr(_build, "INCLUDE", str(include))
+    compiled = []
+
+    def compiler(cmd, **kw):
+        compiled.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(_build.subprocess, "run", compiler)
+    for expected in (1, 1):
+        _build.build_binding()
+        assert len(compiled) == expected
+    (include / "trcuda.h").write_text(text.replace("TRC_CACHE_MAX_WHOLE 512", "TRC_CACHE_MAX_WHOLE 256"))
+    _build.build_binding()
+    assert len(compiled) == 2
+    with open(_build.BINDING_SOURCE) as f:
+        source = f.read()
+    assert "512" not in source and "TRC_CACHE_MAX_WHOLE" in source

@@ -95,8 +95,11 @@ def build_binding(force: bool = False, verbose: bool = False) -> str:
     import torch
 
     root = os.path.dirname(torch.__file__)
-    with open(BINDING_SOURCE, "rb") as f:
-        digest = hashlib.sha256(f.read() + f"{torch.__version__} {sys.version}".encode()).hexdigest()[:16]
+    sources = b""
+    for name in (BINDING_SOURCE, os.path.join(INCLUDE, "trcuda.h")):
+        with open(name, "rb") as f:
+            sources += f.read()
+    digest = hashlib.sha256(sources + f"{torch.__version__} {sys.version}".encode()).hexdigest()[:16]
     stamp = BINDING_PATH + ".hash"
     if not force and os.path.exists(BINDING_PATH) and os.path.exists(stamp):
         with open(stamp) as f:

@@ -18,23 +18,20 @@
 #include <cstring>
 #include <string>
 
+#include "../../include/trcuda.h"
+
 namespace {
 
-using PlanFn = int (*)(const int32_t*, const int32_t*, int, int, const int32_t*, int, int32_t*, int, int, int32_t*,
-                       int32_t*, int32_t*, int32_t*, int32_t*, void*);
-using AppendFn = int (*)(int, const void*, int64_t, int64_t, int, int, int, int, const int32_t*, const int32_t*,
-                         const float*, int, int, void*, int64_t, void*, void*, float*, int*, void*);
-using WorkspaceFn = int64_t (*)(int, int, int);
-using AttentionFn = int (*)(int, const void*, int64_t, const void*, const void*, const int32_t*, int, const int32_t*,
-                            const int32_t*, int, int, int, int, int, int, int, int, int, int, float, const float*,
-                            void*, int64_t, void*, int64_t, int*, void*);
+using PlanFn = decltype(&trc_cache_plan);
+using AppendFn = decltype(&trc_cache_append);
+using WorkspaceFn = decltype(&trc_cache_workspace);
+using AttentionFn = decltype(&trc_cache_attention);
 PlanFn g_plan = nullptr;
 AppendFn g_append = nullptr;
 WorkspaceFn g_workspace = nullptr;
 AttentionFn g_attention = nullptr;
 
 constexpr int64_t kDim = 64;
-constexpr int64_t kMaxWhole = 512;  // TRC_CACHE_MAX_WHOLE
 
 // A failed check: becomes Python's ValueError. A failed library call: becomes TRCError through its code.
 struct Refused {
@@ -308,7 +305,7 @@ PyObject* attention(const Args& a) {
   if (rows) {
     at::Tensor held;  // of the current stream's pool: free for later work on it
     int64_t bytes = 0;
-    if (max_total > kMaxWhole) {
+    if (max_total > TRC_CACHE_MAX_WHOLE) {
       bytes = g_workspace((int)max_new, (int)heads, (int)pool.heads);
       if (bytes < 0) throw Failed{bytes};
       held = at::empty({bytes}, q.options().dtype(at::kByte));
