@@ -155,7 +155,7 @@ int trc_ola_noalloc(const float* d_chunks, int64_t chunk_out_len, const int64_t*
  * allocation and without host synchronisation, so they can be captured in a CUDA graph.
  *
  * A sequence is one stream; its tokens are frames. A frame's query heads are all bands' heads (heads of band 0,
- * then of band 1, ...), any number; cache heads divide them evenly (query head i reads cache head
+ * then of band 1, ...), any number below 2^25; cache heads divide them evenly (query head i reads cache head
  * i / (heads / kv_heads)); head dimension 64. Pools: K and V [n_pages][kv_heads][page][64] 16-bit, page 16, 32,
  * 64 or 128 frames. Block table: int32 [n_seqs][table_stride], entry j the page of frames j * page ...; slot =
  * page number * page + frame within the page. Rows (new frames) of all sequences are packed: sequence i has rows

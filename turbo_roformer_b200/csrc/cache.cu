@@ -695,6 +695,8 @@ int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const 
     return set_last_error(TRC_E_INVALID, "cache attention: bad sizes");
   if (heads / kv_heads > trc::kCacheMaxGroup)
     return set_last_error(TRC_E_INVALID, "cache attention: more than TRC_CACHE_MAX_GROUP query heads per cache head");
+  if (heads > INT_MAX / 64)  // offsets within a row are 32-bit
+    return set_last_error(TRC_E_INVALID, "cache attention: rows of 2^31 elements or more");
   const int lp = trc::page_log2_of(page);
   if (lp < 0) return set_last_error(TRC_E_INVALID, "cache attention: page must be 16, 32, 64 or 128 frames");
   // TMA addresses the pool by rows with 32-bit coordinates, and reads its zero fill just behind it
