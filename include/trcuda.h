@@ -190,7 +190,8 @@ int trc_cache_plan(const int32_t* d_cached, const int32_t* d_new, int n_seqs, in
  * shipped model's). Rotary pairs (2j, 2j + 1) turn by d_positions[row] * d_freqs[j] (fp32 [32], angles in fp64;
  * NULL: no rotation). d_q [n_rows][bands * heads][64], q_stride elements between frames; k and v go to
  * d_slots[row] of the pools (bands * kv_heads cache heads); d_gates [n_rows][bands * heads] fp32 = sigmoid
- * (NULL: none). Rows of slot < 0 are skipped; a slot behind the pool is not written and sets *d_status. Row
+ * (NULL: none). Rows of slot < 0 are skipped; a slot behind the pool is not written and sets *d_status; rows that
+ * name the same slot leave it undefined. Row
  * starts and d_freqs are 16-byte aligned; at most 1,048,560 rows, 4,096 bands and 4,096 heads per band. What is written
  * overlaps nothing else (refused), but with one band d_q may be d_qkv (q_stride = row_stride): q in its place. */
 int trc_cache_append(int precision, const void* d_qkv, int64_t row_stride, int64_t band_stride, int n_rows, int bands,
@@ -210,7 +211,9 @@ int64_t trc_cache_workspace(int max_new, int heads, int kv_heads);
  * between variants and never change which rows and keys are computed. A score of NaN or +inf that a row sees makes the
  * row NaN; one of -inf weighs nothing (a row of such scores only is zero). d_workspace is not used where
  * max_total <= TRC_CACHE_MAX_WHOLE. Frames that a row's masks hide do not change it as long as the cached v are
- * finite; what the pages hold behind `total`, or wholly before every row's window, is not read into any result. d_out
+ * finite; what the pages hold behind `total`, or wholly before every row's window, is not read into any result.
+ * Scores, maxima, sums and norms are fp32; weights are rounded to the 16-bit type for the product with v (half a step
+ * each) and good to 7.5e-5 of themselves before that, as in trc_attention; the result is rounded once. d_out
  * and d_workspace overlap nothing else (refused); d_out may be other columns of the buffer that holds d_q. */
 int trc_cache_attention(int precision, const void* d_q, int64_t q_stride, const void* d_k, const void* d_v,
                         const int32_t* d_table, int table_stride, const int32_t* d_cu, const int32_t* d_total,

@@ -101,8 +101,9 @@ bool overlap(const Rows& a, const Rows& b, int64_t n) {
 // flat ranges: the fresh pages (each finds its sequence by a search in the scan) and the rows, four at a time (one
 // search, then onwards; vector stores). Nothing is exchanged between blocks, so one launch serves any batch: a row's
 // page is either fresh (read from the free list, not from the table that another block is writing) or was in the table
-// before. Lengths and sums sit in shared memory. Bound by the latency of the scan: a push of 8 streams takes 4 us, one
-// of 4,001 sequences and a million rows 11 to 15 us (8.9 MB: 1.4 us of HBM).
+// before. Lengths and sums sit in shared memory. A push of 8 streams takes 4 us, the launch and the scan's latency; one
+// of 4,001 sequences and a million rows 11 to 15 us (8.9 MB: 1.4 us of HBM): 59 % of the issue slots, every row finds
+// its own page.
 struct PlanArgs {
   const int32_t* cached;
   const int32_t* fresh;  // new lengths
@@ -351,7 +352,8 @@ __global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const __gr
     const float fr[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      // half turns: the angle over pi, modulo 2; fp64 keeps 1e-9 of a turn at positions past 2^30
+      // half turns: the angle over pi, modulo 2; fp64 keeps 1e-9 of a turn up to 5e7 frames and 2.6e-8 up to 2^30, as
+      // many bits as an fp64 product position x frequency has
       const double h = pos * (double)fr[p] * 0.31830988618379067154;
       sincospif((float)(h - 2.0 * rint(0.5 * h)), &turn[p].y, &turn[p].x);
     }

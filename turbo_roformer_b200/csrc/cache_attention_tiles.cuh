@@ -24,7 +24,10 @@
 // and end about three steps, a launch 12 us up to its first weights. 1,701 frames x 496 heads: 650 to 680 us under the
 // power cap. A step's time is neither the exponentials' nor the products' alone: without any exponential it is a fifth
 // less, with a quarter of the products the same. It is the chain from S to P to the next product, of which three tiles
-// hide a part (384 rows: issue slots 52 % used, tensor pipe 32 %, MUFU 58 %).
+// hide a part (384 rows: issue slots 52 % used, tensor pipe 32 %, MUFU 58 %). The time attention, which does the same
+// products and exponentials without pages, masks and a divided line, takes 0.89 of this time (1,701 frames x 232
+// heads: 264 and 296 us in turn). Why separate tiles need 40 % more cycles per step than shared ones is not located:
+// each run waits for its one Q buffer, and the softmax has 112 registers instead of 144.
 // Roles: warps 0-2 MMA issuers of tiles 0-2, warp 3 owns TMEM, producers, softmax + epilogue (CtSmem).
 #pragma once
 
@@ -69,7 +72,7 @@ struct CtSmem {
   // Warps 0-2 issue; the producers are warp 3 (shared) or warps 4-6; then twelve softmax warps. Registers per thread
   // after setmaxnreg add up to what the launch gives (checked before it): 512 x 128 = 128 x 80 + 384 x 144, or
   // 640 x 96 = 128 x 72 + 128 x 72 + 384 x 112. The issuers and producers need theirs: with 40 and 56 (128 for the
-  // softmax) they spill inside their loops, and 100 rows over 1,700 frames take 138 instead of 129 us.
+  // softmax) they spill inside their loops, and 100 rows over 1,700 frames take 7 % longer.
   static constexpr int kProducer0 = SHARED ? 3 : 4;
   static constexpr int kSoftmax0 = SHARED ? 4 : 8;
   static constexpr int kThreads = 32 * (kSoftmax0 + 4 * kCtTiles);

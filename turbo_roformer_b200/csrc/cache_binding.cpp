@@ -247,7 +247,8 @@ PyObject* append(const Args& a) {
   at::Tensor gates;
   float* g = nullptr;
   if (wanted) {
-    gates = new_gates ? at::empty({rows, bands * heads}, qkv.options().dtype(at::kFloat)) : plain(a.tensor(9, "gates"), "gates");
+    gates = new_gates ? at::empty({rows, bands * heads}, qkv.options().dtype(at::kFloat))
+                      : plain(a.tensor(9, "gates"), "gates");
     g = gates_of(gates, rows, bands * heads, device);
   }
   if (rows) {

@@ -68,8 +68,8 @@ def cache_plan(cached: torch.Tensor, new: torch.Tensor, table: torch.Tensor, fre
                max_rows: int, out: CachePlan | None = None) -> CachePlan:
     """Pages, slots and positions of a push: ``cached`` and ``new`` (sequences,) int32 frames each sequence has and
     gets. Sequences take the pages they lack from the front of ``free_pages`` into ``table`` (sequences, columns),
-    in place; ``max_rows`` is the capacity of the per-row outputs. ``out``: a plan to write into; its ``total`` is not ``cached``
-    (kept lengths are advanced by ``cached += new`` after the push)."""
+    in place; ``max_rows`` is the capacity of the per-row outputs. ``out``: a plan to write into; its ``total`` is not
+    ``cached`` (kept lengths are advanced by ``cached += new`` after the push)."""
     r = (_binding or _load()).plan(cached, new, table, free_pages, page, max_rows, out)
     return r if r is out else CachePlan._make(r)
 
@@ -85,7 +85,8 @@ def cache_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor
     frequencies (the checkpoint's ``rotary_embed.freqs``), None for no rotation. Returns q (rows, bands * heads,
     64) and the sigmoid gates (rows, bands * heads) fp32, or None; ``q`` and ``gates`` may be tensors to write into
     (``gates=True``: a new one). Rows whose slot is -1 are skipped: where q and gates are new, their values there
-    are undefined. What is written overlaps no other argument; only with one band may ``q`` be the q of ``qkv`` itself."""
+    are undefined. Rows that name the same slot leave it undefined. What is written overlaps no other argument; only
+    with one band may ``q`` be the q of ``qkv`` itself."""
     return (_binding or _load()).append(qkv, positions, slots, k_pages, v_pages, heads, kv_heads, freqs, q, gates,
                                         status)
 
@@ -99,7 +100,11 @@ def cache_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     after it; ``window`` > 0: only that many up to itself. ``gates`` (rows, heads) fp32 scale the result, which is
     zero for a frame that sees nothing. ``max_new`` / ``max_total``: the longest new part and total as far as the
     host knows; they choose the kernel variant only. At most 2,048 sequences: of a longer plan, calls take slices
-    ``table[a:b]``, ``cu[a:b + 1]``, ``total[a:b]`` with the same ``q`` and ``out``. ``out``: where to write (not over another argument); otherwise a new
-    tensor, undefined in rows behind the last sequence's."""
+    ``table[a:b]``, ``cu[a:b + 1]``, ``total[a:b]`` with the same ``q`` and ``out``. ``out``: where to write (not over
+    another argument); otherwise a new tensor, undefined in rows behind the last sequence's.
+
+    Weights are rounded to the 16-bit type for the product with v; scores, sums and norms are fp32. A NaN or +inf
+    score makes its row NaN. A v that is not finite may also make NaN of rows that a mask hides it from, where other
+    rows of their push see it."""
     return (_binding or _load()).attention(q, k_pages, v_pages, table, cu, total, max_new, max_total, causal, window,
                                            scale, gates, out, status)
