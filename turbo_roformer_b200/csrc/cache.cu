@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const __grid_c
     if (column < a.table_stride) a.table[(int64_t)r * a.table_stride + column] = a.free_pages[e];
   }
   // entries that the free list no longer serves, a warp per sequence: the work is the table's, whatever the lengths are
-  if (live_pages > a.n_free) {
+  if (all_pages > a.n_free) {
     for (int r = first >> 5; r < a.n_seqs; r += stride >> 5) {
       int c, n;
       plan_lengths(a, r, c, n);
