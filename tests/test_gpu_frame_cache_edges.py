@@ -112,6 +112,25 @@ def test_infinite_keys(cuda_device, dtype, new):
         assert (np.abs(got - ref)[~up] <= tol[~up]).all(), at
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("new", [1, 3, 20, 100, 300])
+def test_keys_not_finite_in_divided_items(cuda_device, new, value):
+    """Long caches whose keys are divided among workers: a key that is not finite in the first, a middle or the last
+    part makes the rows of its head NaN that score NaN or +inf there, and no others."""
+    total = new + 6000
+    for at in (14, 2999, total - new):
+        c = Case("fp16", [new, 2], [total, 900], 4, 4, 64, seed=1)
+        want = f64(c.run(causal=False))
+        c.k[int(c.table[0, at // 64]), 2, at % 64, 7] = value
+        got, q = f64(c.run(causal=False)), f64(c.q)
+        gone = np.zeros_like(got, bool)
+        gone[:new, 2] = True if value != value else (q[:new, 2, 7] > 0)[:, None]
+        assert np.isnan(got[gone]).all(), at
+        assert np.isfinite(got[~gone]).all(), at
+        other = [0, 1, 3]
+        assert np.array_equal(got[:, other], want[:, other]) and np.array_equal(got[new:], want[new:]), at
+
+
 @pytest.mark.parametrize("dtype,big", [("bf16", 3e38), ("fp16", 65504.0)])
 @pytest.mark.parametrize("new", VARIANTS)
 def test_hidden_values_of_any_finite_size(cuda_device, dtype, big, new):
